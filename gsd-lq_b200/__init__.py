@@ -11,6 +11,8 @@ Modules
   packer    synthetic format-conformant packer (NumPy, and CUDA for big shapes)
   ops       thin wrappers from torch tensors to the C-ABI entry points
   model     GSDLQModel: the reference's load / forward_token / sample_token surface
+  batch     BatchDecoder: lockstep decode of several sequences
+  paged     PagedKV: a paged cache with shared pages; PagedBatchDecoder on top of it
   tp        tensor-parallel sharding of packed linears over NCCL
 """
 __version__ = "0.1.0"

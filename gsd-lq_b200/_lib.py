@@ -21,7 +21,7 @@ GSDLQ_OK = 0
 EPI_STORE, EPI_RESID, EPI_SWIGLU, EPI_ROPE_KV = 0, 1, 2, 3
 IN_PLAIN, IN_RMSNORM, IN_EMBED = 0, 1, 2
 FLAG_NAMES = {0x1: "bad_code", 0x2: "bad_kink", 0x4: "bad_pos", 0x8: "bad_table", 0x10: "timeout",
-              0x20: "bad_token", 0x40: "unsupported", 0x80: "range"}
+              0x20: "bad_token", 0x40: "unsupported", 0x80: "range", 0x100: "bad_page", 0x200: "no_page"}
 
 
 class HexMat(ctypes.Structure):
@@ -61,6 +61,34 @@ class DecodeLayer(ctypes.Structure):
 class DecodeDesc(ctypes.Structure):
     _fields_ = [("n_layers", i32), ("layers", ctypes.POINTER(DecodeLayer)), ("head", LinearJob),
                 ("argmax_key", vp), ("token", vp), ("pos", vp), ("step", vp), ("out_ids", vp), ("max_out", i32)]
+
+
+KV_F16, KV_BF16 = 0, 1
+PAGED_MAX_SEQS = 1024  # GSDLQ_PAGED_MAX_SEQS
+MAX_TOP = 32           # GSDLQ_MAX_TOP
+
+
+class PagedKVDesc(ctypes.Structure):
+    _fields_ = [("k", vp), ("v", vp), ("kv_type", i32), ("layers", i32), ("n_pages", i32), ("page_size", i32),
+                ("n_kv_heads", i32), ("head_dim", i32), ("table", vp), ("refs", vp), ("n_seqs", i32),
+                ("max_blocks", i32)]
+
+
+class PagedAppendJob(ctypes.Structure):
+    _fields_ = [("kv", PagedKVDesc), ("layer", i32), ("q", vp), ("k", vp), ("v", vp), ("q_out", vp),
+                ("q_stride", i32), ("kv_stride", i32), ("q_out_stride", i32), ("rope_cs", vp), ("max_pos", i32),
+                ("interleaved", i32), ("row_seq", vp), ("pos", vp), ("rows", i32), ("n_heads", i32)]
+
+
+class PagedAttnJob(ctypes.Structure):
+    _fields_ = [("kv", PagedKVDesc), ("layer", i32), ("q", vp), ("q_stride", i32), ("out", vp), ("row_seq", vp),
+                ("pos", vp), ("rows", i32), ("n_heads", i32), ("sm_scale", f32), ("work", vp),
+                ("work_bytes", ctypes.c_size_t)]
+
+
+class LogprobsJob(ctypes.Structure):
+    _fields_ = [("logits", vp), ("row_stride", ctypes.c_size_t), ("rows", i32), ("n", i32), ("temperature", f32),
+                ("ids", vp), ("logprob", vp), ("entropy", vp), ("top", i32), ("top_ids", vp), ("top_logprobs", vp)]
 
 
 SIGNATURES = {
@@ -110,6 +138,14 @@ SIGNATURES = {
     "gsdlq_swiglu_rows": ([vp, vp, i32, i32, vp], i32),
     "gsdlq_argmax_rows": ([vp, i32, i32, vp, vp, vp, i32, vp], i32),
     "gsdlq_attention_rows": ([vp] * 5 + [ctypes.c_size_t] + [i32] * 7 + [f32, vp], i32),
+    "gsdlq_rope_kv_paged": ([ctypes.POINTER(PagedAppendJob), vp], i32),
+    "gsdlq_attention_paged_work_size": ([i32, i32, i32, i32, szp], i32),
+    "gsdlq_attention_paged": ([ctypes.POINTER(PagedAttnJob), vp], i32),
+    "gsdlq_pages_fork": ([ctypes.POINTER(PagedKVDesc), vp, vp], i32),
+    "gsdlq_pages_reserve": ([ctypes.POINTER(PagedKVDesc), vp, vp, i32, vp, vp, i32, vp, vp], i32),
+    "gsdlq_pages_compact": ([ctypes.POINTER(PagedKVDesc), vp, vp, i32, vp, vp, ctypes.c_size_t, vp], i32),
+    "gsdlq_pages_copy": ([ctypes.POINTER(PagedKVDesc), vp, vp, vp, i32, vp], i32),
+    "gsdlq_logprobs_rows": ([ctypes.POINTER(LogprobsJob), vp], i32),
 }
 IPC_HANDLE_BYTES = 64
 

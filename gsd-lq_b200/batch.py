@@ -61,9 +61,6 @@ class BatchDecoder:
         dev = m.device
         f32 = dict(dtype=torch.float32, device=dev)
         Lc, kv, hd = m.n_layers, m.n_kv_local, m.head_dim
-        self.k_cache = torch.zeros((B, Lc, S, kv, hd), dtype=torch.float16, device=dev)
-        self.v_cache = torch.zeros_like(self.k_cache)
-        self.seq_stride = Lc * S * kv * hd
         H, F, qd = m.hidden, m.ffn_local, m.n_heads_local * hd
         self.x, self.xn = torch.zeros((B, H), **f32), torch.zeros((B, H), **f32)
         self.q, self.att = torch.zeros((B, qd), **f32), torch.zeros((B, qd), **f32)
@@ -72,7 +69,6 @@ class BatchDecoder:
         self.g, self.u = torch.zeros((B, F), **f32), torch.zeros((B, F), **f32)
         self.logits = torch.zeros((B, m.vocab_local), **f32)
         self.work = ops.matmul_work(B, max(h.cols for h in m.hex.values()), dev)
-        self.awork = ops.attention_rows_work(B, m.n_heads_local, hd, dev)
         self.xy = {r: torch.from_numpy(ops.codebook(r)).to(dev) for r in (6, 8)}
         self.ids = torch.zeros(B, dtype=torch.int32, device=dev)
         self.pos = torch.zeros(B, dtype=torch.int32, device=dev)
@@ -90,6 +86,16 @@ class BatchDecoder:
             self.qkv = torch.zeros((B, qd + 2 * kv * hd), **f32)
             self.gu = torch.zeros((B, 2 * F), **f32)
         self._graph = None
+        self._init_cache()
+
+    def _init_cache(self):
+        """The K/V cache of every sequence and the attention's scratch."""
+        m, B, S = self.m, self.B, self.S
+        Lc, kv, hd = m.n_layers, m.n_kv_local, m.head_dim
+        self.k_cache = torch.zeros((B, Lc, S, kv, hd), dtype=torch.float16, device=m.device)
+        self.v_cache = torch.zeros_like(self.k_cache)
+        self.seq_stride = Lc * S * kv * hd
+        self.awork = ops.attention_rows_work(B, m.n_heads_local, hd, m.device)
 
     # ------------------------------------------------------------------ state
     def prefill(self, b: int, ids, start_pos: int = 0):
@@ -118,13 +124,25 @@ class BatchDecoder:
         h = self.fused[name] if name in self.fused else self.m.hex[name]
         ops.hex2d_matmul(xin, h, self.xy[h.radius], yout, self.work)
 
+    def _attend(self, l, qp, kp, vp, stride):
+        """RoPE and K/V append of the step's rows, then their attention into self.att (layer l; q, k, v at the
+        given addresses, their rows ``stride`` elements apart, 0: packed)."""
+        m, lib, sh = self.m, L.load(), ops.stream_handle()
+        L.check(lib.gsdlq_rope_kv_batch(qp, kp, vp, stride, self.k_cache.data_ptr(), self.v_cache.data_ptr(),
+                                        self.seq_stride, m.rope_cs.data_ptr(), l, self.pos.data_ptr(), self.B,
+                                        m.n_heads_local, m.n_kv_local, m.head_dim, self.S, sh), "gsdlq_rope_kv_batch")
+        L.check(lib.gsdlq_attention_decode_batch(qp, stride, self.k_cache.data_ptr(), self.v_cache.data_ptr(),
+                                                 self.seq_stride, self.att.data_ptr(), self.awork.data_ptr(),
+                                                 self.awork.numel(), l, self.pos.data_ptr(), self.B,
+                                                 m.n_heads_local, m.n_kv_local, m.head_dim, self.S,
+                                                 1.0 / math.sqrt(m.head_dim), sh), "gsdlq_attention_decode_batch")
+
     def _run(self, with_pick: bool = True):
         m, lib, sh = self.m, L.load(), ops.stream_handle()
         B, H, F = self.B, m.hidden, m.ffn_local
         x, xn = self.x, self.xn
         L.check(lib.gsdlq_embed_rows(m.embed.data_ptr(), self.ids.data_ptr(), B, m.vocab_size, H, x.data_ptr(), sh),
                 "gsdlq_embed_rows")
-        sm = 1.0 / math.sqrt(m.head_dim)
         for l in range(m.n_layers):
             p = f"blk.{l}."
             L.check(lib.gsdlq_rmsnorm_rows(x.data_ptr(), m.norms[p + "attn_norm.weight"].data_ptr(), xn.data_ptr(), B,
@@ -139,15 +157,7 @@ class BatchDecoder:
                 self._mm(xn, p + "attn_k.weight", self.k)
                 self._mm(xn, p + "attn_v.weight", self.v)
                 qp, kp, vp, stride = self.q.data_ptr(), self.k.data_ptr(), self.v.data_ptr(), 0
-            L.check(lib.gsdlq_rope_kv_batch(qp, kp, vp, stride, self.k_cache.data_ptr(), self.v_cache.data_ptr(),
-                                            self.seq_stride, m.rope_cs.data_ptr(), l, self.pos.data_ptr(), B,
-                                            m.n_heads_local, m.n_kv_local, m.head_dim, self.S, sh),
-                    "gsdlq_rope_kv_batch")
-            L.check(lib.gsdlq_attention_decode_batch(qp, stride, self.k_cache.data_ptr(),
-                                                     self.v_cache.data_ptr(), self.seq_stride, self.att.data_ptr(),
-                                                     self.awork.data_ptr(), self.awork.numel(), l,
-                                                     self.pos.data_ptr(), B, m.n_heads_local, m.n_kv_local,
-                                                     m.head_dim, self.S, sm, sh), "gsdlq_attention_decode_batch")
+            self._attend(l, qp, kp, vp, stride)
             self._mm(self.att, p + "attn_output.weight", self.o)
             L.check(lib.gsdlq_vec_add(x.data_ptr(), x.data_ptr(), self.o.data_ptr(), B * H, sh), "gsdlq_vec_add")
             L.check(lib.gsdlq_rmsnorm_rows(x.data_ptr(), m.norms[p + "ffn_norm.weight"].data_ptr(), xn.data_ptr(), B,
@@ -193,6 +203,11 @@ class BatchDecoder:
     def logits_host(self) -> np.ndarray:
         """The last step's logits, [B][vocab]."""
         return self.logits.cpu().numpy()
+
+    def logprobs(self, ids=None, top: int = 0, temperature: float = 1.0) -> dict:
+        """Of the last step's logits, per sequence (gsdlq_logprobs_rows): the entropy, the log probability of
+        the given token ids (default: the greedy picks), and the ``top`` most likely tokens with theirs."""
+        return self.m._logprobs(self.logits, self.ids if ids is None else ids, top, temperature)
 
     def generate(self, prompts, max_new_tokens: int) -> list[list[int]]:
         """Greedy continuation of every prompt (prefilled by chunks, then lockstep decode)."""

@@ -7,6 +7,7 @@ CPU path.
 from __future__ import annotations
 
 import ctypes
+import math
 import warnings
 
 import numpy as np
@@ -271,3 +272,147 @@ def attention_ws_size(n_heads, n_kv, hd, max_seq) -> tuple[int, int]:
 
 def attention(job: L.AttnJob):
     L.check(_lib().gsdlq_attention(ctypes.byref(job), stream_handle()), "gsdlq_attention")
+
+
+# ---- paged cache and log probabilities ----------------------------------------------------
+# The calls below take a job (the C descriptor with its tensors checked once and kept alive), as linear() and
+# attention() do: a decode loop builds its jobs at the start and launches them every step.
+def _check(t, name: str, dtype, shape, device, row_stride: bool = False):
+    """A device tensor of the given dtype and shape (None: any size there) on ``device``; contiguous, but for
+    the stride between its rows where ``row_stride``."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
+    if t.device != device or t.device.type != "cuda":
+        raise ValueError(f"{name} must be on the CUDA device of the call ({device}), not on {t.device}")
+    if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    inner = t[0] if row_stride and t.shape[0] else t
+    if not inner.is_contiguous() or (row_stride and t.shape[0] > 1 and t.stride(0) < inner.numel()):
+        raise ValueError(f"{name} must be contiguous" + (" within its rows" if row_stride else ""))
+    return t
+
+
+def _row_stride(t) -> int:
+    return t.stride(0) if t.shape[0] > 1 else 0
+
+
+def _rows(kv, pos, row_seq, device):
+    rows = _check(pos, "pos", torch.int32, (None,), device).numel()
+    if row_seq is not None:
+        _check(row_seq, "row_seq", torch.int32, (rows,), device)
+    if rows < 1 or (row_seq is None and rows > kv.n_seqs):
+        raise ValueError("one row per sequence without row_seq, and at least one")
+    return rows
+
+
+def _on_current(device):
+    if device.index != torch.cuda.current_device():
+        raise ValueError(f"the tensors are on {device}, but cuda:{torch.cuda.current_device()} is the current device")
+
+
+def paged_append_job(kv, layer: int, q, k, v, q_out, pos, rope_cs, row_seq=None, interleaved: bool = True):
+    """Job of rope_kv_paged: q [rows][heads][head_dim], k and v [rows][kv heads][head_dim] (fp32, rows may be
+    strided, k and v alike), q_out like q (or q itself), rope_cs [positions][head_dim / 2][2]."""
+    dev, hd = kv.k.device, kv.head_dim
+    rows = _rows(kv, pos, row_seq, dev)
+    _check(q, "q", torch.float32, (rows, None, hd), dev, row_stride=True)
+    _check(q_out, "q_out", torch.float32, tuple(q.shape), dev, row_stride=True)
+    for t, name in ((k, "k"), (v, "v")):
+        _check(t, name, torch.float32, (rows, kv.n_kv_heads, hd), dev, row_stride=True)
+    if _row_stride(k) != _row_stride(v):
+        raise ValueError("k and v must have the same row stride")
+    _check(rope_cs, "rope_cs", torch.float32, (None, hd // 2, 2), dev)
+    if not 0 <= layer < kv.n_layers:
+        raise ValueError(f"layer outside [0, {kv.n_layers})")
+    j = L.PagedAppendJob(kv=kv.desc(), layer=layer, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(),
+                         q_out=q_out.data_ptr(), q_stride=_row_stride(q), kv_stride=_row_stride(k),
+                         q_out_stride=_row_stride(q_out), rope_cs=rope_cs.data_ptr(), max_pos=rope_cs.shape[0],
+                         interleaved=int(interleaved), row_seq=None if row_seq is None else row_seq.data_ptr(),
+                         pos=pos.data_ptr(), rows=rows, n_heads=q.shape[1])
+    j.keep, j.device = (kv, q, k, v, q_out, pos, rope_cs, row_seq), dev
+    return j
+
+
+def rope_kv_paged(job):
+    """RoPE of the job's rows and their k and v into their pages (gsdlq_rope_kv_paged)."""
+    _on_current(job.device)
+    L.check(_lib().gsdlq_rope_kv_paged(ctypes.byref(job), stream_handle()), "gsdlq_rope_kv_paged")
+
+
+def attention_paged_work(kv, rows: int, n_heads: int) -> torch.Tensor:
+    """A zeroed work area for attention_paged of up to ``rows`` rows (one per launch that may overlap)."""
+    n = ctypes.c_size_t()
+    L.check(_lib().gsdlq_attention_paged_work_size(rows, n_heads, kv.n_kv_heads, kv.head_dim, ctypes.byref(n)),
+            "attention_paged_work_size")
+    return torch.zeros(int(n.value), dtype=torch.uint8, device=kv.k.device)
+
+
+def paged_attn_job(kv, layer: int, q, out, pos, sm_scale: float, work, row_seq=None):
+    """Job of attention_paged: q [rows][heads][head_dim] fp32 (rows may be strided), out the same shape, packed."""
+    dev, hd = kv.k.device, kv.head_dim
+    rows = _rows(kv, pos, row_seq, dev)
+    _check(q, "q", torch.float32, (rows, None, hd), dev, row_stride=True)
+    _check(out, "out", torch.float32, tuple(q.shape), dev)
+    _check(work, "work", torch.uint8, (None,), dev)
+    if not 0 <= layer < kv.n_layers:
+        raise ValueError(f"layer outside [0, {kv.n_layers})")
+    if q.shape[1] < 1 or q.shape[1] % kv.n_kv_heads:
+        raise ValueError("the query heads must be a multiple of the kv heads")
+    if not math.isfinite(sm_scale):
+        raise ValueError("sm_scale must be finite")
+    if q.data_ptr() % 16 or _row_stride(q) % 4:
+        raise ValueError("q and its rows must start at multiples of 16 bytes")
+    j = L.PagedAttnJob(kv=kv.desc(), layer=layer, q=q.data_ptr(), q_stride=_row_stride(q), out=out.data_ptr(),
+                       row_seq=None if row_seq is None else row_seq.data_ptr(), pos=pos.data_ptr(), rows=rows,
+                       n_heads=q.shape[1], sm_scale=sm_scale, work=work.data_ptr(), work_bytes=work.numel())
+    j.keep, j.device = (kv, q, out, pos, work, row_seq), dev
+    return j
+
+
+def attention_paged(job):
+    """Attention of the job's rows over their sequences' pages (gsdlq_attention_paged)."""
+    _on_current(job.device)
+    L.check(_lib().gsdlq_attention_paged(ctypes.byref(job), stream_handle()), "gsdlq_attention_paged")
+
+
+def logprobs_job(logits, ids=None, logprob=None, entropy=None, top_ids=None, top_logprobs=None,
+                 temperature: float = 1.0):
+    """Job of logprobs_rows: logits [rows][n] fp32 (rows may be strided); ids int32 [rows] with logprob [rows];
+    entropy [rows]; top_ids int32 and top_logprobs [rows][top].  What is None is not computed."""
+    if not isinstance(logits, torch.Tensor):
+        raise TypeError("logits must be a tensor")
+    dev = logits.device
+    _check(logits, "logits", torch.float32, (None, None), dev, row_stride=True)
+    rows, n = logits.shape
+    if rows < 1 or n < 1:
+        raise ValueError("logits must have at least one row and one column")
+    if (ids is None) != (logprob is None) or (top_ids is None) != (top_logprobs is None):
+        raise ValueError("ids and logprob, and top_ids and top_logprobs, go together")
+    if ids is None and entropy is None and top_ids is None:
+        raise ValueError("nothing to compute")
+    for t, name, dt in ((ids, "ids", torch.int32), (logprob, "logprob", torch.float32),
+                        (entropy, "entropy", torch.float32)):
+        if t is not None:
+            _check(t, name, dt, (rows,), dev)
+    top = 0
+    if top_ids is not None:
+        top = _check(top_ids, "top_ids", torch.int32, (rows, None), dev).shape[1]
+        _check(top_logprobs, "top_logprobs", torch.float32, (rows, top), dev)
+        if top > min(n, L.MAX_TOP):
+            raise ValueError(f"at most {min(n, L.MAX_TOP)} alternatives")
+    if not (temperature > 0.0 and math.isfinite(temperature)):
+        raise ValueError("temperature must be positive and finite")
+    opt = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    j = L.LogprobsJob(logits=logits.data_ptr(), row_stride=_row_stride(logits), rows=rows, n=n,
+                      temperature=temperature, ids=opt(ids), logprob=opt(logprob), entropy=opt(entropy), top=top,
+                      top_ids=opt(top_ids), top_logprobs=opt(top_logprobs))
+    j.keep, j.device = (logits, ids, logprob, entropy, top_ids, top_logprobs), dev
+    return j
+
+
+def logprobs_rows(job):
+    """Log probabilities, entropy and top alternatives of the job's rows (gsdlq_logprobs_rows)."""
+    _on_current(job.device)
+    L.check(_lib().gsdlq_logprobs_rows(ctypes.byref(job), stream_handle()), "gsdlq_logprobs_rows")

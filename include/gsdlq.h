@@ -47,6 +47,9 @@ extern "C" {
 #define GSDLQ_FLAG_UNSUPPORTED 0x40u /* a kernel found a device limit it was not built for and did nothing */
 #define GSDLQ_FLAG_RANGE 0x80u     /* a low-rank partial sum left the +-2^22 fixed-point range (clamped), or
                                       a scale above 5 reached the batched linear's fp16 weight parts */
+#define GSDLQ_FLAG_BAD_PAGE 0x100u /* a page table entry, page list entry, parent or sequence index outside its
+                                      range, or a page that is missing or shared where it must be written: skipped */
+#define GSDLQ_FLAG_NO_PAGE 0x200u  /* the page pool is exhausted: a row got no page */
 
 typedef void *gsdlq_stream_t;
 
@@ -433,6 +436,129 @@ int gsdlq_attention_decode_batch(const float *q, int q_stride, const uint16_t *k
 int gsdlq_swiglu_rows(const float *gate_up, float *out, int rows, int n, gsdlq_stream_t stream);
 int gsdlq_argmax_rows(const float *logits, int rows, int n, int *ids, int *pos, int *out_ids, int out_stride,
                       gsdlq_stream_t stream);
+
+/* ---- Paged cache: a batch of sequences over one pool of pages -----------------------------------
+ * No counterpart in the reference (one sequence, one contiguous cache).  A pool holds pages of
+ * page_size positions, for every layer, in fp16 or bf16; a sequence's positions j * page_size ..
+ * live in the page table[s][j] (the same page index in every layer's pool), and refs[p] counts the
+ * table entries that name page p (0: the page is free).  Pages may be shared between sequences; a
+ * page is written only while one entry names it.  Tables, counts and positions stay on the device,
+ * so a captured decode step allocates, copies and frees pages without the host.
+ *
+ * Rows: the per-row calls take `rows` new tokens.  Row r belongs to sequence row_seq[r] (row_seq
+ * NULL: sequence r) and stands at position pos[r]; pos[r] = -1 is an idle row (nothing is stored,
+ * its attention output is zero).  One row per sequence is a decode step; consecutive positions of
+ * one sequence are a chunk of its prompt.  Positions below -1 or at max_blocks * page_size and
+ * above set GSDLQ_FLAG_BAD_POS, sequence indices outside [0, n_seqs) GSDLQ_FLAG_BAD_PAGE; such rows
+ * are treated as idle.  Arrays of one call must not overlap unless said so. */
+#define GSDLQ_KV_F16 0
+#define GSDLQ_KV_BF16 1
+#define GSDLQ_PAGED_MAX_SEQS 1024 /* largest n_seqs, and largest rows of gsdlq_pages_reserve */
+
+typedef struct gsdlq_paged_kv {
+  void *k, *v;      /* [layers][n_pages][page_size][n_kv_heads][head_dim], 16-byte aligned            */
+  int kv_type;      /* GSDLQ_KV_F16, GSDLQ_KV_BF16                                                    */
+  int layers, n_pages, page_size, n_kv_heads, head_dim; /* n_pages <= 2^28, page_size >= 1, head_dim 32, 64, 128 */
+  int *table;       /* [n_seqs][max_blocks]; -1: no page                                              */
+  int *refs;        /* [n_pages]                                                                      */
+  int n_seqs, max_blocks;
+} gsdlq_paged_kv_t;
+
+/* RoPE of row r's q and k at pos[r], and k (rotated) and v into its page, rounded to the cache's
+ * type: gsd_cpu_rope_and_store_kv (gsd_lq_cpu_engine.c:186-262) per row, with fp32 arithmetic that
+ * does not contract products and sums.  A row whose page is missing or named by more than one table
+ * entry stores nothing (GSDLQ_FLAG_BAD_PAGE); its q is rotated all the same.  Idle rows' q is copied.
+ * Rows of one call at the same position of one sequence leave an unspecified mixture of their values there. */
+typedef struct gsdlq_paged_append_job {
+  gsdlq_paged_kv_t kv;
+  int layer;
+  const float *q, *k, *v; /* rows of [n_heads][head_dim] and [n_kv_heads][head_dim]                   */
+  float *q_out;           /* rotated q; may be q itself (same stride)                                 */
+  int q_stride, kv_stride, q_out_stride; /* elements between rows; 0: packed                          */
+  const float *rope_cs;   /* [max_pos][head_dim/2] (cos, sin) pairs                                   */
+  int max_pos;            /* positions at and above it: GSDLQ_FLAG_BAD_POS, treated as idle           */
+  int interleaved;        /* 1: pairs (2i, 2i+1); 0: (i, i + head_dim/2)                              */
+  const int *row_seq, *pos;
+  int rows, n_heads;
+} gsdlq_paged_append_job_t;
+int gsdlq_rope_kv_paged(const gsdlq_paged_append_job_t *job, gsdlq_stream_t stream);
+
+/* Attention of each row's query heads over positions 0 .. pos[r] of its sequence:
+ * out[r][h] = sum_t p_t V[t], p = softmax_t(sm_scale * q[r][h] . K[t]), with kv head
+ * h / (n_heads / n_kv_heads) -- gsd_cpu_gqa_attention (gsd_lq_cpu_engine.c:265-330) per row.  Any
+ * n_heads that is a multiple of n_kv_heads.  Positions whose page is missing are left out
+ * (GSDLQ_FLAG_BAD_PAGE); a row with no position left gives zeros.  Cache rows in use and q must be
+ * finite; what lies behind pos[r] in a page is never used, whatever it holds.
+ * work: gsdlq_attention_paged_work_size bytes, 16-byte aligned, all zero before its first use; each
+ * launch leaves it as it needs it.  Launches that may overlap in time need a work area each. */
+typedef struct gsdlq_paged_attn_job {
+  gsdlq_paged_kv_t kv;
+  int layer;
+  const float *q;      /* rows of [n_heads][head_dim], 16-byte aligned */
+  int q_stride;        /* elements between rows, a multiple of 4; 0: packed */
+  float *out;          /* [rows][n_heads][head_dim], 16-byte aligned */
+  const int *row_seq, *pos;
+  int rows, n_heads;
+  float sm_scale;
+  void *work;
+  size_t work_bytes;
+} gsdlq_paged_attn_job_t;
+int gsdlq_attention_paged_work_size(int rows, int n_heads, int n_kv_heads, int head_dim, size_t *bytes);
+int gsdlq_attention_paged(const gsdlq_paged_attn_job_t *job, gsdlq_stream_t stream);
+
+/* Page lists: src[i] and dst[i] are pages, *counts (device) the number of pairs. */
+
+/* Sequence b takes over the pages of sequence parent[b] (all of them at once, as the table was before
+ * the call), which are then shared; parent[b] = b keeps, -1 frees sequence b's pages.  Forks, frees
+ * and reorders sequences in one call.  refs follows: a page that no entry names any more is free.
+ * A parent outside [-1, n_seqs): GSDLQ_FLAG_BAD_PAGE, the sequence is kept. */
+int gsdlq_pages_fork(const gsdlq_paged_kv_t *kv, const int *parent, gsdlq_stream_t stream);
+
+/* A page to write to for every row's position.  Row by row, in order: a missing page is replaced by a
+ * free one; a page that other entries name too is replaced by a free one that is to receive its
+ * contents, and the pair goes on the list; a page of one's own is kept.  Free pages are taken in
+ * ascending order.  When none is left the row's entry stays as it is (GSDLQ_FLAG_NO_PAGE).
+ * counts[0] = pairs, counts[1] = rows that got no page, counts[2] = pages taken; list entries from
+ * counts[0] up to max_pairs are -1.  max_pairs >= rows, rows <= GSDLQ_PAGED_MAX_SEQS. */
+int gsdlq_pages_reserve(const gsdlq_paged_kv_t *kv, const int *row_seq, const int *pos, int rows, int *src, int *dst,
+                        int max_pairs, int *counts, gsdlq_stream_t stream);
+
+/* Renumber pages so that those in use come first: the highest page in use moves to the lowest free
+ * one, and so on, until the pages in use are 0 .. n - 1 or max_pairs pages have moved.  Tables and
+ * refs are rewritten; the pairs on the list are still to be copied (no page is on both sides).
+ * counts[0] = pairs, counts[1] = pages in use, counts[2] = 1 + the highest page in use afterwards;
+ * list entries from counts[0] on are -1.  work: n_pages ints. */
+int gsdlq_pages_compact(const gsdlq_paged_kv_t *kv, int *src, int *dst, int max_pairs, int *counts, void *work,
+                        size_t work_bytes, gsdlq_stream_t stream);
+
+/* Copy page src[i] over page dst[i] in every layer, K and V, for i < min(*counts, max_pairs).  Pairs with a
+ * page outside the pool are skipped (GSDLQ_FLAG_BAD_PAGE).  A page must not be a destination twice, nor a
+ * source and a destination: the contents of such pages are unspecified. */
+int gsdlq_pages_copy(const gsdlq_paged_kv_t *kv, const int *src, const int *dst, const int *counts, int max_pairs,
+                     gsdlq_stream_t stream);
+
+/* ---- Log probabilities -----------------------------------------------------------------------------
+ * Of rows of logits, with the sampler's rules (NaN -> -1e4, +-inf -> 100 / -1e4, z = logits /
+ * max(temperature, 1e-4); gsd_lq_cpu_runtime.py:422-434): log p_i = z_i - log sum_j exp z_j;
+ *   logprob[r]  = log p of token ids[r] (ids NULL: not computed; ids[r] = -1: 0; outside [-1, n):
+ *                 GSDLQ_FLAG_BAD_TOKEN and 0)
+ *   entropy[r]  = -sum_i p_i log p_i (NULL: not computed)
+ *   top_ids[r][j], top_logprobs[r][j], j < top: the largest log p in descending order, equal ones by
+ *                 ascending index.  0 <= top <= min(n, GSDLQ_MAX_TOP)
+ * temperature > 0 and finite.  row_stride: elements between rows, 0: packed. */
+#define GSDLQ_MAX_TOP 32
+typedef struct gsdlq_logprobs_job {
+  const float *logits;
+  size_t row_stride;
+  int rows, n;
+  float temperature;
+  const int *ids;
+  float *logprob, *entropy;
+  int top;
+  int *top_ids;
+  float *top_logprobs;
+} gsdlq_logprobs_job_t;
+int gsdlq_logprobs_rows(const gsdlq_logprobs_job_t *job, gsdlq_stream_t stream);
 
 /* ---- The whole decode step in one launch ----------------------------------------------------
  * Engine-level entry point with no single reference counterpart: the reference's

@@ -1,0 +1,474 @@
+"""The paged cache's operators on the GPU (gsdlq_rope_kv_paged, gsdlq_attention_paged, gsdlq_pages_*) against
+plain restatements (paged_oracle.py): page bookkeeping and stored rows exactly, attention within a bound derived
+there.  Everything of a pool that no position uses is NaN, so that a read of it shows."""
+import math
+
+import numpy as np
+import pytest
+
+import paged_oracle as O
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+DTYPES = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def flags():
+    import gsdlq_b200._lib as L
+    return L.flag_names(L.device_flags())
+
+
+def dev(a, dtype=torch.int32):
+    return torch.tensor(a, dtype=dtype, device="cuda")
+
+
+def make_pool(rng, lens, page, nkv, hd, dtype, layers=1, spare=3, max_blocks=None):
+    """Sequences of the given lengths over shuffled pages; all else NaN."""
+    from gsdlq_b200 import paged
+    blocks = [-(-n // page) for n in lens]
+    n_pages, mb = sum(blocks) + spare, max_blocks or max(blocks) + 1
+    perm = rng.permutation(n_pages)
+    table = np.full((len(lens), mb), -1, np.int64)
+    refs = np.zeros(n_pages, np.int64)
+    k = torch.full((layers, n_pages, page, nkv, hd), math.nan, dtype=dtype)
+    v = k.clone()
+    at = 0
+    for s, (n, b) in enumerate(zip(lens, blocks)):
+        table[s, :b] = perm[at:at + b]
+        refs[perm[at:at + b]] = 1
+        for j in range(b):
+            m = min(page, n - j * page)
+            for t in (k, v):
+                t[:, perm[at + j], :m] = torch.from_numpy(rng.standard_normal((layers, m, nkv, hd))).to(dtype)
+        at += b
+    return paged.PagedKV.wrap(k.cuda(), v.cuda(), dev(table), dev(refs))
+
+
+def rows_of(kv, layer, seq, n):
+    """K and V of a sequence's first n positions, as float64."""
+    out = []
+    for t in (kv.k, kv.v):
+        pages = kv.table[seq, :-(-n // kv.page_size)].long()
+        out.append(t[layer, pages].flatten(0, 1)[:n].double().cpu().numpy())
+    return out
+
+
+def run_attention(kv, layer, q, pos, row_seq=None, scale=None):
+    from gsdlq_b200 import ops
+    rows, heads, hd = q.shape
+    guard = torch.full((rows + 1, heads, hd), 77.0, device="cuda")
+    job = ops.paged_attn_job(kv, layer, q, guard[:rows], dev(pos), scale or 1.0 / math.sqrt(hd),
+                             ops.attention_paged_work(kv, rows, heads), None if row_seq is None else dev(row_seq))
+    ops.attention_paged(job)
+    first = guard[:rows].clone()
+    ops.attention_paged(job)  # the work area serves the next launch, with the same result
+    assert torch.equal(first, guard[:rows]) and bool((guard[rows] == 77.0).all())
+    return first.cpu().numpy()
+
+
+def check_attention(kv, layer, q, pos, row_seq=None, scale=None):
+    got = run_attention(kv, layer, q, pos, row_seq, scale)
+    for r, p in enumerate(pos):
+        k, v = rows_of(kv, layer, r if row_seq is None else row_seq[r], p + 1)
+        want, tol = O.attention(q[r].cpu().numpy(), k, v, scale or 1.0 / math.sqrt(q.shape[2]))
+        err = np.abs(got[r] - want)
+        assert (err <= tol).all(), (r, p, float((err - tol).max()), float(err.max()))
+        if p < 0:
+            assert not got[r].any()
+    assert flags() == []
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("hd,nkv,group,page", [
+    (128, 2, 4, 16), (128, 1, 1, 64), (64, 4, 1, 16), (64, 2, 3, 5), (32, 3, 8, 1), (128, 2, 6, 100), (64, 1, 12, 24),
+    (32, 7, 1, 32), (128, 1, 17, 48)])
+def test_attention_lengths_groups_and_pages(cuda_lib, rng, kind, hd, nkv, group, page):
+    lens = [1, 2, 15, 16, 17, 0, 31, 33, 63, 64, 65, 0, 127, 130, 257, 600]
+    kv = make_pool(rng, lens, page, nkv, hd, DTYPES[kind], layers=2)
+    q = torch.from_numpy(rng.standard_normal((len(lens), nkv * group, hd)) * 2).float().cuda()
+    check_attention(kv, 1, q, [n - 1 for n in lens])
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attention_single_rows_over_long_caches(cuda_lib, rng, kind):
+    for hd, nkv, group, n in ((128, 1, 4, 9001), (64, 3, 2, 4097), (32, 1, 5, 7000), (128, 8, 4, 1537)):
+        kv = make_pool(rng, [n], 16, nkv, hd, DTYPES[kind])
+        q = torch.from_numpy(rng.standard_normal((1, nkv * group, hd)) * 2).float().cuda()
+        for pos in (n - 1, n // 2, 0):
+            check_attention(kv, 0, q, [pos])
+
+
+def test_attention_chunk_rows_and_repeated_sequences(cuda_lib, rng):
+    """Consecutive positions of one sequence, rows of several sequences in any order, and the same row twice."""
+    kv = make_pool(rng, [300, 40], 16, 2, 128, torch.float16)
+    rows = [(0, 290 + i) for i in range(10)] + [(1, 3), (0, 7), (1, 39), (1, -1), (0, 7)]
+    q = torch.from_numpy(rng.standard_normal((len(rows), 12, 128)) * 2).float().cuda()
+    q[14] = q[11]
+    pos, seq = [p for _, p in rows], [s for s, _ in rows]
+    check_attention(kv, 0, q, pos, seq)
+    got = run_attention(kv, 0, q, pos, seq)
+    assert np.array_equal(got[11], got[14])
+
+
+def test_attention_strided_q_and_extreme_scores(cuda_lib, rng):
+    kv = make_pool(rng, [50, 200, 7], 16, 2, 64, torch.float16)
+    wide = torch.from_numpy(rng.standard_normal((3, 4 * 64 + 20))).float().cuda()
+    q = wide[:, :256].unflatten(1, (4, 64))
+    check_attention(kv, 0, q, [49, 199, 6])
+    # one position far ahead of the others, scores of some hundreds, tiny queries and zero queries
+    q = q.contiguous()
+    q[0] *= 200.0
+    q[1] *= 1e-30
+    q[2] = 0.0
+    check_attention(kv, 0, q, [49, 199, 6])
+    check_attention(kv, 0, q, [49, 199, 6], scale=-0.25)
+
+
+def test_attention_leaves_out_missing_pages(cuda_lib, rng):
+    """A table entry outside the pool: its positions are left out and reported; no position left: zeros."""
+    kv = make_pool(rng, [64, 64, 16], 16, 1, 64, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((3, 2, 64))).float().cuda()
+    k, v = rows_of(kv, 0, 0, 64)
+    keep = np.r_[0:16, 32:64]
+    kv.table[0, 1] = -1
+    kv.table[1] = torch.tensor([kv.n_pages, -7, 1 << 30, -(1 << 31)] + [-1] * (kv.max_blocks - 4), dtype=torch.int32)
+    got = run_attention(kv, 0, q, [63, 63, 15])
+    want, tol = O.attention(q[0].cpu().numpy(), k[keep], v[keep], 0.125)
+    assert (np.abs(got[0] - want) <= tol).all() and not got[1].any()
+    k, v = rows_of(kv, 0, 2, 16)
+    want, tol = O.attention(q[2].cpu().numpy(), k, v, 0.125)
+    assert (np.abs(got[2] - want) <= tol).all()
+    assert flags() == ["bad_page"]
+    # positions and sequences out of range are idle rows, and reported
+    assert not run_attention(kv, 0, q, [-2, kv.max_blocks * 16, 2**31 - 1]).any()
+    assert flags() == ["bad_pos"]
+    assert not run_attention(kv, 0, q, [3, 3, 3], [-1, 3, 2**31 - 1]).any()
+    assert flags() == ["bad_page"]
+
+
+def test_attention_offsets_past_32_bits(cuda_lib, rng):
+    """Pages whose elements lie more than 2^32 behind the start of the pool."""
+    from gsdlq_b200 import paged
+    page, nkv, hd = 64, 8, 128
+    n_pages = (1 << 32) // (page * nkv * hd) + 40
+    k = torch.empty((1, n_pages, page, nkv, hd), dtype=torch.bfloat16, device="cuda")
+    v = torch.empty_like(k)
+    kv = paged.PagedKV.wrap(k, v, dev([[n_pages - 1, 3, n_pages - 30]]), dev(np.zeros(n_pages, np.int64)))
+    for p in (n_pages - 1, 3, n_pages - 30):
+        for t in (k, v):
+            t[0, p] = torch.from_numpy(rng.standard_normal((page, nkv, hd))).to(torch.bfloat16)
+    q = torch.from_numpy(rng.standard_normal((1, 32, hd))).float().cuda()
+    check_attention(kv, 0, q, [170])
+    kv.refs[n_pages - 30] = 1
+    append_check(kv, 0, rng, [190], 32)
+    kv.counts[0] = 1
+    kv.copy_pages(dev([n_pages - 1]), dev([5]), kv.counts)
+    assert torch.equal(k[0, 5], k[0, n_pages - 1]) and flags() == []
+
+
+# ---------------------------------------------------------------------------------------- append
+def append_check(kv, layer, rng, pos, heads, row_seq=None, interleaved=True, strided=False, in_place=False,
+                 stored=None, max_pos=None):
+    """Append random rows; the whole pool and q must be what the restatement gives (rows in ``stored`` are stored,
+    by default those that are not idle)."""
+    from gsdlq_b200 import ops
+    rows, nkv, hd = len(pos), kv.n_kv_heads, kv.head_dim
+    width = (heads + 2 * nkv) * hd
+    qkv = torch.from_numpy(rng.standard_normal((rows, width + (12 if strided else 0)))).float().cuda()
+    parts = [t.unflatten(1, (-1, hd)) for t in qkv[:, :width].split((heads * hd, nkv * hd, nkv * hd), 1)]
+    q, k, v = parts if strided else [t.contiguous() for t in parts]
+    want_q, nk, nv = (t.cpu().numpy().copy() for t in (q, k, v))
+    cs = rng.standard_normal((max_pos or kv.max_blocks * kv.page_size, hd // 2, 2)).astype(np.float32)
+    before = [t.clone() for t in (kv.k, kv.v)]
+    out = q if in_place else torch.full_like(q, 5.0)
+    ops.rope_kv_paged(ops.paged_append_job(kv, layer, q, k, v, out, dev(pos), torch.from_numpy(cs).cuda(),
+                                           None if row_seq is None else dev(row_seq), interleaved))
+    for r, p in enumerate(pos):
+        s = r if row_seq is None else row_seq[r]
+        if not 0 <= p < cs.shape[0] or p >= kv.max_blocks * kv.page_size or not 0 <= s < kv.n_seqs:
+            continue
+        want_q[r] = O.rotate(want_q[r], cs[p], interleaved)
+        if stored is not None and r not in stored:
+            continue
+        page, o = int(kv.table[s, p // kv.page_size]), p % kv.page_size
+        before[0][layer, page, o] = torch.from_numpy(O.rotate(nk[r], cs[p], interleaved)).to(kv.k.dtype)
+        before[1][layer, page, o] = torch.from_numpy(nv[r]).to(kv.k.dtype)
+    assert np.array_equal(out.cpu().numpy(), want_q)
+    for got, want in zip((kv.k, kv.v), before):
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("hd,nkv,heads,page", [(128, 2, 8, 16), (64, 32, 32, 24), (32, 3, 9, 1), (64, 5, 15, 64)])
+def test_append_rows(cuda_lib, rng, kind, hd, nkv, heads, page):
+    lens = [1, 33, 16, 5, 17, 64]
+    kv = make_pool(rng, lens, page, nkv, hd, DTYPES[kind], layers=2)
+    pos = [n - 1 for n in lens]
+    pos[3] = -1
+    append_check(kv, 1, rng, pos, heads)
+    append_check(kv, 0, rng, pos, heads, strided=True)
+    append_check(kv, 0, rng, pos, heads, interleaved=False, in_place=True)
+    append_check(kv, 1, rng, [60, 61, 62, 63, 2], heads, row_seq=[5, 5, 5, 5, 1], strided=True, in_place=True)
+    assert flags() == []
+
+
+def test_append_refuses_shared_and_missing_pages(cuda_lib, rng):
+    kv = make_pool(rng, [20, 20, 20, 20], 16, 2, 64, torch.float16)
+    kv.refs[int(kv.table[0, 1])] = 2   # shared
+    kv.table[1, 1] = -1                # missing
+    kv.table[2, 1] = kv.n_pages        # outside the pool
+    append_check(kv, 0, rng, [19] * 4, 4, stored=[3])
+    assert flags() == ["bad_page"]
+    append_check(kv, 0, rng, [-1, -5, kv.max_blocks * 16, 5], 4)
+    assert flags() == ["bad_pos"]
+    append_check(kv, 0, rng, [3, 12, 3, 11], 4, max_pos=12)  # the table of angles ends at 12
+    assert flags() == ["bad_pos"]
+    append_check(kv, 0, rng, [3, 3, 3], 4, row_seq=[4, -1, 3])
+    assert flags() == ["bad_page"]
+
+
+def test_append_rounds_overflow_and_ties_as_the_type_does(cuda_lib, rng):
+    from gsdlq_b200 import ops
+    for dtype in DTYPES.values():
+        kv = make_pool(rng, [16], 16, 1, 32, dtype)
+        v = torch.tensor([65504.0, 65519.9, 65520.0, -1e30, 1e-8, 2.0**-24, 2.0**-25, 1.0 + 2.0**-11,
+                          1.0 + 3 * 2.0**-11, 1.0 + 2.0**-8, 1.0 + 3 * 2.0**-8, 3.4e38, math.inf, -math.inf, 0.0, -0.0]
+                         * 2, device="cuda").reshape(1, 1, 32)
+        q = torch.zeros(1, 1, 32, device="cuda")
+        cs = torch.zeros(16, 16, 2, device="cuda")
+        cs[..., 0] = 1.0
+        ops.rope_kv_paged(ops.paged_append_job(kv, 0, q, q.clone(), v, q.clone(), dev([15]), cs))
+        got = kv.v[0, int(kv.table[0, 0]), 15, 0]
+        assert torch.equal(got.view(torch.int16), v[0, 0].to(dtype).view(torch.int16))
+
+
+# ---------------------------------------------------------------------------------------- pages
+def empty_pool(n_pages, page, seqs, blocks, layers=2, dtype=torch.float16):
+    """Every page of every layer holds values of its own."""
+    from gsdlq_b200 import paged
+    kv = paged.PagedKV(layers, n_pages, page, 2, 32, seqs, blocks, dtype)
+    for t, sign in ((kv.k, 1), (kv.v, -1)):
+        p = torch.arange(layers * n_pages, device="cuda").reshape(layers, n_pages, 1, 1, 1)
+        t += (sign * (p % 997) + torch.arange(2 * 32, device="cuda").reshape(1, 1, 1, 2, 32) / 64).to(dtype)
+    return kv
+
+
+def same(kv, want, pools):
+    assert kv.table.tolist() == want.table
+    assert kv.refs.tolist() == want.refs
+    for got, exp in zip((kv.k, kv.v), pools):
+        assert torch.equal(got, exp)
+
+
+def test_pages_random_sequences_of_operations(cuda_lib, rng):
+    """Forks, reservations and compactions in random order on a pool that now and then runs out."""
+    seqs, blocks, page, n_pages = 9, 11, 4, 40
+    kv = empty_pool(n_pages, page, seqs, blocks)
+    want = O.Pages(kv.table.tolist(), kv.refs.tolist(), page)
+    pools = [kv.k.clone(), kv.v.clone()]
+
+    def moved(pairs, counts, most):
+        assert kv.counts[:3].tolist() == counts
+        assert kv.src[:most].tolist() == [a for a, _ in pairs] + [-1] * (most - len(pairs))
+        assert kv.dst[:most].tolist() == [b for _, b in pairs] + [-1] * (most - len(pairs))
+        for t in pools:
+            t[:, [b for _, b in pairs]] = t[:, [a for a, _ in pairs]].clone()
+
+    ran_out = 0
+    for step in range(150):
+        what = rng.integers(0, 10)
+        if what < 6:
+            n = int(rng.integers(1, 3 * seqs))
+            rows = [(int(rng.integers(0, seqs)), int(rng.integers(-1, blocks * page))) for _ in range(n)]
+            kv.reserve(dev([p for _, p in rows]), dev([s for s, _ in rows]))
+            pairs, failed, taken = want.reserve(rows)
+            moved(pairs, [len(pairs), failed, taken], n)
+            ran_out += failed > 0
+            assert flags() == (["no_page"] if failed else [])
+        elif what < 9:
+            parent = [int(rng.choice([b, b, b, -1, rng.integers(0, seqs)])) for b in range(seqs)]
+            kv.fork(dev(parent))
+            want.fork(parent)
+        else:
+            most = int(rng.integers(1, 12))
+            kv.compact(most)
+            pairs, live, high = want.compact(most)
+            moved(pairs, [len(pairs), live, high], most)
+        same(kv, want, pools)
+    assert ran_out > 3 and flags() == []
+
+
+@pytest.mark.parametrize("n_pages", [1, 31, 4095, 4096, 4097, 20000])
+def test_pages_large_pools_and_many_rows(cuda_lib, rng, n_pages):
+    """Pools over several scan steps; free pages far apart; a thousand rows."""
+    from gsdlq_b200 import paged
+    seqs, blocks = 1024, 8
+    refs = (rng.random(n_pages) < 0.7).astype(np.int64)
+    kv = paged.PagedKV(1, n_pages, 2, 1, 32, seqs, blocks)
+    kv.k += torch.arange(n_pages, device="cuda").reshape(1, -1, 1, 1, 1) % 1999
+    live = np.flatnonzero(refs)
+    flat = np.full(seqs * blocks, -1)
+    flat[:min(len(live), flat.size)] = rng.permutation(live)[:flat.size]
+    table = rng.permutation(flat).reshape(seqs, blocks)
+    kv.table.copy_(dev(table))
+    kv.refs.copy_(dev(refs))
+    want = O.Pages(table, refs, 2)
+    pools = [kv.k.clone(), kv.v.clone()]
+    pos = [int(p) for p in rng.integers(-1, blocks * 2, seqs)]
+    kv.reserve(dev(pos))
+    pairs, failed, taken = want.reserve(list(enumerate(pos)))
+    assert kv.counts[:3].tolist() == [len(pairs), failed, taken]
+    same(kv, want, pools)
+    kv.fork(dev([b // 2 if b % 3 else -1 for b in range(seqs)]))
+    want.fork([b // 2 if b % 3 else -1 for b in range(seqs)])
+    same(kv, want, pools)
+    kv.compact()
+    # the restatement's compaction, done at once
+    live = [p for p, r in enumerate(want.refs) if r > 0]
+    n = len(live)
+    src = [p for p in reversed(live) if p >= n]
+    dst = [p for p in range(n) if want.refs[p] <= 0]
+    to = dict(zip(src, dst))
+    want.table = [[to.get(e, e) for e in r] for r in want.table]
+    for a, b in zip(src, dst):
+        want.refs[b], want.refs[a] = want.refs[a], 0
+        for t in pools:
+            t[:, b] = t[:, a]
+    assert kv.counts[:3].tolist() == [len(src), n, n]
+    same(kv, want, pools)
+    flags()  # (small pools run out)
+
+
+def test_pages_bad_entries_are_reported_and_harmless(cuda_lib):
+    kv = empty_pool(10, 4, 4, 3)
+    kv.reserve(dev([0, 5, 2, -1]))
+    assert kv.table.tolist() == [[0, -1, -1], [-1, 1, -1], [2, -1, -1], [-1, -1, -1]]
+    kv.fork(dev([0, 4, -2, 0]))  # parents out of range: kept
+    assert kv.table.tolist() == [[0, -1, -1], [-1, 1, -1], [2, -1, -1], [0, -1, -1]]
+    assert flags() == ["bad_page"] and kv.refs.tolist()[:4] == [2, 1, 1, 0]
+    kv.table[2, 0] = 99  # an entry outside the pool counts as missing
+    kv.reserve(dev([0, -1, 1, -1]))
+    assert flags() == ["bad_page"]
+    assert kv.counts[:3].tolist() == [1, 0, 2]
+    assert kv.table.tolist()[0][0] == 3 and kv.table.tolist()[2][0] == 4
+    kv.reserve(dev([12, -9, 2**31 - 1]))
+    assert flags() == ["bad_pos"] and kv.counts[:3].tolist() == [0, 0, 0]
+    kv.reserve(dev([0, 0]), dev([4, -1]))
+    assert flags() == ["bad_page"] and kv.counts[:3].tolist() == [0, 0, 0]
+    before = kv.k.clone()
+    counts = dev([3])
+    kv.copy_pages(dev([0, 10, -1]), dev([7, 2, 3]), counts)
+    want = before.clone()
+    want[:, 7] = before[:, 0]
+    assert torch.equal(kv.k, want) and flags() == ["bad_page"]
+    for n in (0, -5):  # nothing to copy
+        kv.copy_pages(dev([1]), dev([2]), dev([n]))
+        assert torch.equal(kv.k, want)
+    kv.copy_pages(dev([1]), dev([8]), dev([1000]))  # a count past the list: the list's length holds
+    want[:, 8] = want[:, 1]
+    assert torch.equal(kv.k, want) and flags() == []
+
+
+def test_resized_pool(cuda_lib):
+    kv = empty_pool(12, 4, 3, 3)
+    kv.reserve(dev([0, 4, 8]))
+    kv.reserve(dev([0, 0, 0]))
+    kv.fork(dev([-1, 1, 2]))
+    with pytest.raises(ValueError):
+        kv.resized(3)
+    kv.compact()
+    n = kv.pages_in_use()
+    assert kv.counts[:3].tolist() == [1, n, n]
+    small = kv.resized(n)
+    assert torch.equal(small.k, kv.k[:, :n]) and torch.equal(small.v, kv.v[:, :n]) and small.n_pages == n
+    assert torch.equal(small.refs, kv.refs[:n]) and small.table is kv.table
+    big = small.resized(30)
+    assert torch.equal(big.k[:, :n], small.k) and big.refs.tolist() == small.refs.tolist() + [0] * (30 - n)
+    big.reserve(dev([0, -1, -1]))
+    assert big.table[0, 0] == n and flags() == []
+
+
+# ---------------------------------------------------------------------------------------- as they are used
+def test_steps_captured_in_graphs_on_two_streams(cuda_lib, rng):
+    """Reserve, append and attention captured and replayed, two caches with a work area each on two streams at
+    once, against the eager calls on the default stream."""
+    from gsdlq_b200 import ops, paged
+    heads, nkv, hd, page, seqs = 8, 2, 64, 4, 3
+    cs = torch.from_numpy(rng.standard_normal((64, hd // 2, 2))).float().cuda()
+
+    def setup(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        kv = paged.PagedKV(1, 60, page, nkv, hd, seqs, 16)
+        kv.k.fill_(math.nan)
+        kv.v.fill_(math.nan)
+        x = torch.randn(40, seqs, (heads + 2 * nkv), hd, generator=g, device="cuda")
+        cur, pos = x[0].clone(), dev([0, -1, 0])
+        out = torch.zeros(seqs, heads, hd, device="cuda")
+        q = torch.zeros(seqs, heads, hd, device="cuda")
+        append = ops.paged_append_job(kv, 0, cur[:, :heads], cur[:, heads:heads + nkv], cur[:, heads + nkv:], q, pos, cs)
+        attn = ops.paged_attn_job(kv, 0, q, out, pos, 0.125, ops.attention_paged_work(kv, seqs, heads))
+
+        def step():
+            kv.reserve(pos)
+            ops.rope_kv_paged(append)
+            ops.attention_paged(attn)
+            pos.add_((pos >= 0).int())
+        return kv, x, cur, pos, out, step
+
+    steps = 30
+    plain = []
+    for seed in (1, 2):
+        kv, x, cur, pos, out, step = setup(seed)
+        res = []
+        for i in range(steps):
+            cur.copy_(x[i])
+            step()
+            res.append(out.clone())
+        plain.append((torch.stack(res), kv.table.clone(), kv.refs.clone()))
+    runs = []
+    for seed in (1, 2):
+        kv, x, cur, pos, out, step = setup(seed)
+        torch.cuda.synchronize()
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            step()  # warm-up; its position is taken back
+            pos.sub_((pos >= 0).int())
+            g = torch.cuda.CUDAGraph()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(g, stream=st):
+                step()
+        runs.append((kv, x, cur, out, g, st, []))
+    torch.cuda.synchronize()
+    for i in range(steps):
+        for kv, x, cur, out, g, st, res in runs:
+            with torch.cuda.stream(st):
+                cur.copy_(x[i])
+                g.replay()
+                res.append(out.clone())
+    torch.cuda.synchronize()
+    for (want, table, refs), (kv, _, _, _, _, _, res) in zip(plain, runs):
+        assert torch.equal(torch.stack(res), want)
+        assert torch.equal(kv.table, table) and torch.equal(kv.refs, refs)
+    assert flags() == []
+
+
+def test_fork_then_write_keeps_the_others_rows(cuda_lib, rng):
+    """Fork, reserve, append, attention: each copy sees the shared prefix and its own new row."""
+    from gsdlq_b200 import ops
+    kv = make_pool(rng, [21, 0, 0, 0], 8, 2, 64, torch.float16, spare=8, max_blocks=5)
+    kv.fork(dev([0, 0, 0, -1]))
+    kv.reserve(dev([21, 21, 21, -1]))
+    assert kv.counts[:3].tolist() == [2, 0, 2]
+    old_k, old_v = rows_of(kv, 0, 2, 21)
+    append_check(kv, 0, rng, [21, 21, 21, -1], 4)
+    last = []
+    for s in range(3):
+        k, v = rows_of(kv, 0, s, 22)
+        assert np.array_equal(k[:21], old_k) and np.array_equal(v[:21], old_v)
+        last.append(k[21])
+    assert not np.array_equal(last[0], last[1]) and not np.array_equal(last[1], last[2])
+    q = torch.from_numpy(rng.standard_normal((4, 4, 64))).float().cuda()
+    check_attention(kv, 0, q, [21, 21, 21, -1])
+    kv.fork(dev([-1, -1, -1, -1]))
+    assert not kv.refs.any() and (kv.table == -1).all() and flags() == []
