@@ -560,9 +560,10 @@ class GSDLQModel:
             self._pf = b
         return b
 
-    def _prefill_chunk(self, ids, pos0: int, k_cache=None, v_cache=None, max_seq: int | None = None):
+    def _prefill_chunk(self, ids, pos0: int, k_cache=None, v_cache=None, max_seq: int | None = None, attend=None):
         """One chunk of batched prefill into (k_cache, v_cache) ([layers][max_seq][kv heads][head_dim]
-        fp16; the model's own cache by default)."""
+        fp16; the model's own cache by default).  attend(l, b): appends and attends layer l's rows b["q"],
+        b["k"], b["v"] into b["att"] over a cache of the caller's instead."""
         lib, sh = L.load(), ops.stream_handle()
         b = self._prefill_bufs()
         kc = self.k_cache if k_cache is None else k_cache
@@ -584,13 +585,17 @@ class GSDLQModel:
             mm(xn, p + "attn_q.weight", b["q"])
             mm(xn, p + "attn_k.weight", b["k"])
             mm(xn, p + "attn_v.weight", b["v"])
-            L.check(lib.gsdlq_rope_kv_rows(b["q"].data_ptr(), b["k"].data_ptr(), b["v"].data_ptr(), kc.data_ptr(),
-                                           vc.data_ptr(), self.rope_cs.data_ptr(), l, pos0, n, self.n_heads_local,
-                                           self.n_kv_local, self.head_dim, S, sh), "gsdlq_rope_kv_rows")
-            L.check(lib.gsdlq_attention_rows(b["q"].data_ptr(), kc.data_ptr(), vc.data_ptr(), b["att"].data_ptr(),
-                                             b["awork"].data_ptr(), b["awork"].numel(), l, pos0, n,
-                                             self.n_heads_local, self.n_kv_local, self.head_dim, S, sm, sh),
-                    "gsdlq_attention_rows")
+            if attend is not None:
+                attend(l, b)
+            else:
+                L.check(lib.gsdlq_rope_kv_rows(b["q"].data_ptr(), b["k"].data_ptr(), b["v"].data_ptr(), kc.data_ptr(),
+                                               vc.data_ptr(), self.rope_cs.data_ptr(), l, pos0, n,
+                                               self.n_heads_local, self.n_kv_local, self.head_dim, S, sh),
+                        "gsdlq_rope_kv_rows")
+                L.check(lib.gsdlq_attention_rows(b["q"].data_ptr(), kc.data_ptr(), vc.data_ptr(),
+                                                 b["att"].data_ptr(), b["awork"].data_ptr(), b["awork"].numel(), l,
+                                                 pos0, n, self.n_heads_local, self.n_kv_local, self.head_dim, S, sm,
+                                                 sh), "gsdlq_attention_rows")
             mm(b["att"], p + "attn_output.weight", b["o"])
             L.check(lib.gsdlq_vec_add(x.data_ptr(), x.data_ptr(), b["o"].data_ptr(), n * H, sh), "gsdlq_vec_add")
             L.check(lib.gsdlq_rmsnorm_rows(x.data_ptr(), self.norms[p + "ffn_norm.weight"].data_ptr(), xn.data_ptr(),
@@ -601,6 +606,59 @@ class GSDLQModel:
                     "gsdlq_swiglu")
             mm(b["g"], p + "ffn_down.weight", b["o"])
             L.check(lib.gsdlq_vec_add(x.data_ptr(), x.data_ptr(), b["o"].data_ptr(), n * H, sh), "gsdlq_vec_add")
+
+    def _logprobs(self, logits, ids, top: int, temperature: float) -> dict:
+        """gsdlq_logprobs_rows over device logits [rows][vocab]; ids: per row a token id, -1 for none."""
+        rows, dev = logits.shape[0], logits.device
+        if not isinstance(ids, torch.Tensor):
+            ids = torch.tensor([int(i) for i in ids], dtype=torch.int32)
+        if ids.numel() != rows:
+            raise ValueError("one token id per row")
+        if not 0 <= top <= min(logits.shape[1], L.MAX_TOP):
+            raise ValueError(f"top outside [0, {min(logits.shape[1], L.MAX_TOP)}]")
+        ids = ids.to(dev, torch.int32)
+        f32 = dict(dtype=torch.float32, device=dev)
+        out = {"logprob": torch.empty(rows, **f32), "entropy": torch.empty(rows, **f32),
+               "top_ids": torch.empty((rows, top), dtype=torch.int32, device=dev),
+               "top_logprobs": torch.empty((rows, top), **f32)}
+        ops.logprobs_rows(ops.logprobs_job(logits, ids=ids, temperature=temperature, **out))
+        return {k: v.cpu().numpy() for k, v in out.items()}
+
+    def logprobs(self, ids=(-1,), top: int = 0, temperature: float = 1.0) -> dict:
+        """Of the last step's logits: the entropy, the log probability of one token id (-1: none), and the
+        ``top`` most likely tokens with theirs (arrays of one row)."""
+        if self.tp is not None:
+            raise NotImplementedError("log probabilities need the whole vocabulary on one GPU")
+        return self._logprobs(self.logits[None], ids, top, temperature)
+
+    def score(self, ids, top: int = 0, temperature: float = 1.0) -> dict:
+        """Log probabilities of a token sequence under the model: row i holds the log probability of
+        ids[i + 1] after ids[: i + 1] (0 in the last row, which has no next token), the entropy there, and
+        the ``top`` most likely next tokens.  Runs the chunks of prefill, each with the LM head and
+        gsdlq_logprobs_rows over its rows, so the cache holds the sequence afterwards."""
+        if self.tp is not None or not self.batched_prefill_supported:
+            raise NotImplementedError("scoring runs on one GPU, for the shapes of batched prefill")
+        ids = [int(t) for t in ids]
+        if not ids or len(ids) > self.max_seq:
+            raise ValueError(f"between 1 and {self.max_seq} tokens")
+        if min(ids) < 0 or max(ids) >= self.vocab_size:
+            raise ValueError("token id outside the vocabulary")
+        if getattr(self, "_score_logits", None) is None:
+            self._score_logits = torch.zeros((self.PREFILL_CHUNK, self.vocab_size), dtype=torch.float32,
+                                             device=self.device)
+        parts = []
+        for c in range(0, len(ids), self.PREFILL_CHUNK):
+            chunk = ids[c:c + self.PREFILL_CHUNK]
+            self._prefill_chunk(chunk, c)
+            b, n, head = self._prefill_bufs(), len(chunk), self.hex["output.weight"]
+            L.check(L.load().gsdlq_rmsnorm_rows(b["x"].data_ptr(), self.norms["output_norm.weight"].data_ptr(),
+                                                b["xn"].data_ptr(), n, self.hidden, self.rms_eps,
+                                                ops.stream_handle()), "gsdlq_rmsnorm_rows")
+            logits = self._score_logits[:n]
+            ops.hex2d_matmul(b["xn"][:n], head, b["xy"][head.radius], logits, b["work"])
+            nxt = ids[c + 1:c + n + 1]
+            parts.append(self._logprobs(logits, nxt + [-1] * (n - len(nxt)), top, temperature))
+        return {k: np.concatenate([p[k] for p in parts]) for k in parts[0]}
 
     def generate(self, prompt_ids, max_new_tokens: int, temperature: float = 0.0, top_p: float = 0.9,
                  eos_id: int | None = None, check_every: int = 16, start_pos: int = 0,
