@@ -71,23 +71,6 @@ __device__ __forceinline__ void ldsm_x2_trans(uint32_t addr, uint32_t& b0, uint3
                : "memory");
 }
 
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-// the address of the same shared-memory variable in CTA `rank` of this cluster
-__device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
-}
-
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 // Sums 16 values over the 32 lanes of a warp in 16 shuffles (instead of 16 x 5): after the
 // exchanges lane l holds the total of value (l >> 1) & 15.
 __device__ __forceinline__ float warp_sum16(float (&v)[16], int lane) {
