@@ -8,6 +8,7 @@
 // Leaving the maximum's own 1 out of S keeps peaked rows exact: where S is far below 1, log(1 + S) in fp32
 // would lose S to the rounding of 1 + S.
 #include <cfloat>
+#include <climits>
 #include <cmath>
 
 #include "common.cuh"
@@ -17,15 +18,16 @@ namespace gsdlq {
 // A row is read once, by a cluster of 1 to 8 CTAs that each take a contiguous part of it.  A thread keeps the
 // maximum m of its logits, and of the others the sums s of e^u and t of u e^u with u = (x - m) / temperature (in
 // units of ln 2): a logit above m costs a rescaling and pushes the old maximum into the sums, every other one an
-// ex2 and two additions.  Partial results (m1 >= m2) join as
+// ex2 and two additions.  Logits come in batches, so that lanes with a new maximum diverge once per batch.  Partial results (m1 >= m2) join as
 //   d = (m2 - m1) / temperature,  f = e^d,  s = s1 + f (s2 + 1),  t = t1 + f (t2 + d (s2 + 1)).
 //
-// Alternatives without a second pass over the row: the threads' own maxima come with their indices, the maxima of
-// the 64 groups of eight threads are ranked, and every token of the row's top k has a key of at least the k-th
-// largest group maximum, K, since k tokens have; and it lies in one of the k groups whose maximum is at least K.
-// Only those groups' tokens are looked at again (they are in the L2 cache), those at or above K -- mostly a few
-// more than k -- are collected and ranked by counting.  Keys are (z, lowest index first) with z as the sampler
-// rounds it, so equal z (different logits can share one) go by index.
+// Alternatives without a second pass over the row: the maxima of the 64 groups of eight threads are ranked.  Every
+// token of the best k has a key of at least the k-th largest group maximum, K, since k tokens have; and it lies in
+// one of the k groups whose maximum is at least K.  Only those groups' tokens are looked at again (they are in the
+// L2 cache); those at or above K -- mostly a few more than k -- are collected and ranked by counting.  Keys are
+// (z, lowest index first) with z as the sampler rounds it, so equal z (different logits can share one) go by index;
+// the groups' indices are looked up only where the k-th maximum is shared by more groups than are wanted, as in
+// rows with fewer unmasked tokens than k.
 constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_GROUPS = LP_THREADS / 8;      // >= GSDLQ_MAX_TOP
 constexpr int LP_CAP = 1280;                   // tokens collected before the slow path takes over
@@ -40,11 +42,14 @@ struct LpShared {
   LpSums part;                  // this CTA's
   int n_top;                    // entries of top: k, or fewer where the CTA's part is shorter
   lp_key_t top[GSDLQ_MAX_TOP];  // this CTA's best, in order
-  lp_key_t group[LP_GROUPS];
+  uint32_t gz[LP_GROUPS], kz;  // the groups' maxima, and the k-th largest of them
+  int over;                    // how many of the groups that share it are wanted, where not all are
+  lp_key_t group[LP_GROUPS];   // their keys then
   lp_key_t K, red[LP_WARPS];
   lp_key_t all[LP_MAX_CLUSTER][GSDLQ_MAX_TOP];
   LpSums parts[LP_MAX_CLUSTER];
   int counts[LP_MAX_CLUSTER];
+  int n_list, list[GSDLQ_MAX_TOP];  // the groups that hold the CTA's best
   int found;
   lp_key_t cand[LP_CAP];
 };
@@ -80,32 +85,55 @@ __device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b, float c) {
 
 struct LpThread {
   LpSums a;
-  float near;  // logits at or above it are looked at closely
-  float z;     // the best z, and its first index
-  int i;
+  float near;    // a batch whose maximum reaches it may hold a better z
+  float z;       // the best z (-inf: nothing yet) ...
+  int at, vecs;  // ... and the batch that holds its first index: `vecs` vectors from `at` on
 };
-__device__ __forceinline__ void lp_add(LpThread& T, float x, int i, float temp, float c) {
-  x = lp_clean(x);
-  if (x >= T.near) {
-    const float z = lp_z(x, temp);
+constexpr int LP_HEAD = -1, LP_TAIL = -2;  // `at` of the single logits before and behind the vectors
+
+// N logits in the order of their indices.  A new maximum changes places with the old one, so that what is added
+// to the sums is again everything but the maximum.  (Lanes that find one wait for nobody more than once per batch;
+// logit by logit nearly every one is a new maximum in some lane.)
+template <int N>
+__device__ __forceinline__ void lp_add(LpThread& T, float (&x)[N], int at, int vecs, float temp, float c) {
+  float wild = 0.f;  // not finite if a logit is not
+#pragma unroll
+  for (int k = 0; k < N; ++k) wild = fmaf(x[k], 0.f, wild);
+  if (wild != 0.f) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) x[k] = lp_clean(x[k]);
+  }
+  float top = x[0];
+#pragma unroll
+  for (int k = 1; k < N; ++k) top = fmaxf(top, x[k]);
+  if (top >= T.near) {
+    const float z = lp_z(top, temp);
     if (z > T.z) {
       T.z = z;
-      T.i = i;
+      T.at = at;
+      T.vecs = vecs;
     }
-    if (x > T.a.m) {
-      if (T.a.m != -INFINITY) {
-        const float d = fmaxf((T.a.m - x) * c, -200.f), f = lp_ex2(d), s1 = T.a.s + 1.f;
-        T.a.t = f * fmaf(d, s1, T.a.t);
-        T.a.s = f * s1;
+    if (top > T.a.m) {
+      const float f = lp_ex2(fmaxf((T.a.m - top) * c, -200.f)), d = fmaxf((T.a.m - top) * c, -200.f);
+      T.a.t = f * fmaf(d, T.a.s, T.a.t);
+      T.a.s *= f;
+      bool placed = false;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const bool it = !placed && x[k] == top;
+        placed |= it;
+        x[k] = it ? T.a.m : x[k];  // -inf at first, which adds nothing
       }
-      T.a.m = x;
-      T.near = lp_below(x);
-      return;
+      T.a.m = top;
+      T.near = lp_below(top);
     }
   }
-  const float d = fmaxf((x - T.a.m) * c, -200.f), e = lp_ex2(d);
-  T.a.s += e;
-  T.a.t = fmaf(e, d, T.a.t);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float d = fmaxf((x[k] - T.a.m) * c, -200.f), e = lp_ex2(d);
+    T.a.s += e;
+    T.a.t = fmaf(e, d, T.a.t);
+  }
 }
 
 __device__ lp_key_t lp_block_max(LpShared& S, lp_key_t k) {
@@ -134,25 +162,32 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
   const int v0 = lo + head, nv = (hi - v0) / 4, tail = hi - v0 - 4 * nv;
   const float4* const xv = reinterpret_cast<const float4*>(x + v0);
 
-  LpThread T = {{-INFINITY, 0.f, 0.f}, -INFINITY, -INFINITY, 0};
-  if (tid < head) lp_add(T, x[lo + tid], lo + tid, temp, c);
-  constexpr int UN = 4;
-  for (int v = tid; v < nv; v += UN * LP_THREADS) {
-    float4 w[UN];
-#pragma unroll
-    for (int k = 0; k < UN; ++k)
-      if (v + k * LP_THREADS < nv) w[k] = __ldg(xv + v + k * LP_THREADS);
-#pragma unroll
-    for (int k = 0; k < UN; ++k)
-      if (v + k * LP_THREADS < nv) {
-        const int i = v0 + 4 * (v + k * LP_THREADS);
-        lp_add(T, w[k].x, i, temp, c);
-        lp_add(T, w[k].y, i + 1, temp, c);
-        lp_add(T, w[k].z, i + 2, temp, c);
-        lp_add(T, w[k].w, i + 3, temp, c);
-      }
+  // the given token's logit, early
+  const int id = rank == 0 && tid == 0 && J.ids ? J.ids[r] : -1;
+  const float x_id = id >= 0 && id < J.n ? x[id] : 0.f;
+
+  LpThread T = {{-INFINITY, 0.f, 0.f}, -INFINITY, -INFINITY, 0, 0};
+  if (tid < head) {
+    float w[1] = {x[lo + tid]};
+    lp_add<1>(T, w, LP_HEAD, 0, temp, c);
   }
-  if (tid < tail) lp_add(T, x[v0 + 4 * nv + tid], v0 + 4 * nv + tid, temp, c);
+  constexpr int UN = 4;  // vectors of a batch, one every LP_THREADS
+  int v = tid;
+  for (; v + (UN - 1) * LP_THREADS < nv; v += UN * LP_THREADS) {
+    float w[4 * UN];
+#pragma unroll
+    for (int k = 0; k < UN; ++k) *reinterpret_cast<float4*>(w + 4 * k) = __ldg(xv + v + k * LP_THREADS);
+    lp_add<4 * UN>(T, w, v, UN, temp, c);
+  }
+  for (; v < nv; v += LP_THREADS) {
+    float w[4];
+    *reinterpret_cast<float4*>(w) = __ldg(xv + v);
+    lp_add<4>(T, w, v, 1, temp, c);
+  }
+  if (tid < tail) {
+    float w[1] = {x[v0 + 4 * nv + tid]};
+    lp_add<1>(T, w, LP_TAIL, 0, temp, c);
+  }
 
   // ---- sums of the CTA's part
   LpSums a = T.a;
@@ -161,15 +196,16 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
     a = lp_join(a, {__shfl_down_sync(0xffffffffu, a.m, o), __shfl_down_sync(0xffffffffu, a.s, o),
                     __shfl_down_sync(0xffffffffu, a.t, o)}, c);
   if (lane == 0) S.sums[warp] = a;
+  const uint32_t my_z = T.z == -INFINITY ? 0u : ordered_key(T.z);  // 0: no token
   if (J.top > 0) {
-    lp_key_t g = T.z == -INFINITY ? 0ull : lp_key(T.z, T.i);
+    uint32_t g = my_z;
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if ((lane & 7) == 0) S.group[tid >> 3] = g;
+    if ((lane & 7) == 0) S.gz[tid >> 3] = g;
   }
   if (tid == 0) {
-    S.K = 0ull;
-    S.found = 0;
+    S.kz = 0u;
+    S.over = S.found = S.n_list = 0;
   }
   __syncthreads();
   if (warp == 0) {
@@ -185,14 +221,55 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
   if (J.top > 0) {
     const int k = min(J.top, hi - lo);
     if (tid < LP_GROUPS) {
-      const lp_key_t g = S.group[tid];
-      int above = 0;
-#pragma unroll 8
-      for (int j = 0; j < LP_GROUPS; ++j) above += S.group[j] > g;
-      if (above == k - 1 && g != 0ull) S.K = g;  // the keys of groups with tokens differ: one thread
+      const uint32_t g = S.gz[tid];
+      int above = 0, same = 0, first = 0;
+#pragma unroll 16
+      for (int j = 0; j < LP_GROUPS; ++j) {
+        above += S.gz[j] > g;
+        same += S.gz[j] == g;
+        first += S.gz[j] == g && j < tid;
+      }
+      if (above < k && g != 0u) {
+        if (above + same > k) {  // more groups share this maximum than belong to the best k
+          if (first == 0) S.over = k - above;
+        } else {
+          S.list[atomicAdd(&S.n_list, 1)] = tid;
+        }
+        if (above + same >= k) S.kz = g;  // (the same value from all that write it)
+      }
     }
     __syncthreads();
-    const lp_key_t K = S.K;  // 0: fewer groups than k have tokens, and all tokens are collected
+    // the k-th largest group maximum; 0: fewer groups than k have tokens, and all tokens are collected
+    lp_key_t K = (lp_key_t)S.kz << 32;
+    if (S.over > 0) {  // (uniform) of the groups that share it, those with the lowest indices
+      lp_key_t g = 0ull;
+      if (my_z == S.kz && S.gz[tid >> 3] == S.kz) {
+        int i = T.at == LP_HEAD ? lo + tid : v0 + 4 * nv + tid;
+        if (T.at >= 0) {
+          i = INT_MAX;
+          for (int q = 0; q < T.vecs; ++q) {
+            const float4 w = __ldg(xv + T.at + q * LP_THREADS);
+            const float e[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (lp_z(lp_clean(e[j]), temp) == T.z) i = min(i, v0 + 4 * (T.at + q * LP_THREADS) + j);
+          }
+        }
+        g = lp_key(T.z, i);
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if ((lane & 7) == 0) S.group[tid >> 3] = g;
+      __syncthreads();
+      if (tid < LP_GROUPS && S.group[tid] != 0ull) {
+        int above = 0;
+        for (int j = 0; j < LP_GROUPS; ++j) above += S.group[j] > S.group[tid];
+        if (above < S.over) S.list[atomicAdd(&S.n_list, 1)] = tid;
+        if (above == S.over - 1) S.K = S.group[tid];
+      }
+      __syncthreads();
+      K = S.K;
+    }
     const float zk = K ? key_to_float((uint32_t)(K >> 32)) : -INFINITY;
     const float close = K ? lp_below(zk * temp) : -INFINITY;
     auto look = [&](float v, int i) {
@@ -205,21 +282,31 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
         }
       }
     };
-    for (int g = warp; g < LP_GROUPS; g += LP_WARPS) {
-      const lp_key_t key = S.group[g];
-      if (key == 0ull || key < K) continue;
-      for (int v = g * 8 + (lane & 7) + (lane >> 3) * LP_THREADS; v < nv; v += 4 * LP_THREADS) {
-        const float4 w = __ldg(xv + v);
-        const int i = v0 + 4 * v;
-        look(w.x, i);
-        look(w.y, i + 1);
-        look(w.z, i + 2);
-        look(w.w, i + 3);
+    // the listed groups' vectors, dealt to all threads, LOOKS loads at a time
+    constexpr int LOOKS = 4;
+    const int per_group = 8 * ((nv + LP_THREADS - 1) / LP_THREADS), looks = S.n_list * per_group;
+    for (int e0 = tid; e0 < looks; e0 += LOOKS * LP_THREADS) {
+      float4 w[LOOKS];
+      int at[LOOKS];
+#pragma unroll
+      for (int u = 0; u < LOOKS; ++u) {
+        const int e = e0 + u * LP_THREADS, g = e / per_group, j = e - g * per_group;
+        at[u] = e < looks ? S.list[g] * 8 + (j & 7) + (j >> 3) * LP_THREADS : nv;
+        if (at[u] < nv) w[u] = __ldg(xv + at[u]);
       }
-      if (g == 0) {  // the single logits belong to the first threads
-        if (lane < head) look(x[lo + lane], lo + lane);
-        if (lane < tail) look(x[v0 + 4 * nv + lane], v0 + 4 * nv + lane);
-      }
+#pragma unroll
+      for (int u = 0; u < LOOKS; ++u)
+        if (at[u] < nv) {
+          const int i = v0 + 4 * at[u];
+          look(w[u].x, i);
+          look(w[u].y, i + 1);
+          look(w[u].z, i + 2);
+          look(w[u].w, i + 3);
+        }
+    }
+    if (tid < max(head, tail)) {  // the single logits belong to the first threads
+      if (tid < head) look(x[lo + tid], lo + tid);
+      if (tid < tail) look(x[v0 + 4 * nv + tid], v0 + 4 * nv + tid);
     }
     __syncthreads();
     const int found = S.found;
@@ -271,13 +358,12 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
   LpSums row = cluster > 1 ? S.parts[0] : S.part;
   for (int q = 1; q < cluster; ++q) row = lp_join(row, S.parts[q], c);
   const float ls = log1pf(row.s), inv = 1.0f / temp;
-  auto logp = [&](float v) { return (v - row.m) * inv - ls; };
+  const float zm = lp_z(row.m, temp);
   if (tid == 0) {
     if (J.ids) {
-      const int id = J.ids[r];
       float lp = 0.f;
       if (id >= 0 && id < J.n)
-        lp = logp(lp_clean(x[id]));
+        lp = (lp_clean(x_id) - row.m) * inv - ls;
       else if (id != -1)
         raise_flag(GSDLQ_FLAG_BAD_TOKEN);
       J.logprob[r] = lp;
@@ -285,9 +371,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
     if (J.entropy) J.entropy[r] = ls - 0.6931471805599453f * row.t / (1.0f + row.s);
   }
   auto put = [&](int j, lp_key_t key) {
-    const int i = lp_index(key);
-    J.top_ids[(size_t)r * J.top + j] = i;
-    J.top_logprobs[(size_t)r * J.top + j] = logp(lp_clean(x[i]));
+    J.top_ids[(size_t)r * J.top + j] = lp_index(key);
+    J.top_logprobs[(size_t)r * J.top + j] = (key_to_float((uint32_t)(key >> 32)) - zm) - ls;
   };
   if (cluster == 1) {
     if (tid < J.top) put(tid, S.top[tid]);
@@ -327,9 +412,9 @@ extern "C" int gsdlq_logprobs_rows(const gsdlq_logprobs_job_t* job, gsdlq_stream
   if (J.top < 0 || J.top > GSDLQ_MAX_TOP || J.top > J.n || (J.top > 0 && (!J.top_ids || !J.top_logprobs)))
     return GSDLQ_ERR_INVALID;
   if (!J.ids && !J.entropy && J.top == 0) return GSDLQ_ERR_INVALID;
-  // CTAs a row: enough for about four an SM, none with less than 2048 logits
+  // CTAs a row: as many as run at once, two an SM, none with less than 2048 logits
   int cluster = 1;
-  while (cluster < LP_MAX_CLUSTER && (long long)J.rows * cluster * 2 <= 4 * num_sms() && J.n / (cluster * 2) >= 2048)
+  while (cluster < LP_MAX_CLUSTER && (long long)J.rows * cluster * 2 <= 2 * num_sms() && J.n / (cluster * 2) >= 2048)
     cluster *= 2;
   if ((long long)J.rows * cluster > INT32_MAX) return GSDLQ_ERR_INVALID;
   cudaLaunchConfig_t cfg = {};

@@ -81,6 +81,21 @@ def test_equal_logits_and_many_ties(cuda_lib, rng):
         assert np.array_equal(got["top_ids"][0], np.arange(32)) and np.array_equal(got["top_ids"][1], np.arange(32))
 
 
+def test_alternatives_crowded_in_one_place(cuda_lib, rng):
+    """Thousands of tokens above all others, in rows that a block or a cluster reads so that a few threads hold them
+    all; and rows with fewer unmasked tokens than alternatives."""
+    for rows, n, part in ((1, 400000, 50000), (300, 151936, 151936)):
+        x = torch.from_numpy(rng.standard_normal((rows, n)).astype(np.float32)).cuda()
+        i = torch.arange(n, device="cuda") % part
+        x += 100.0 * ((i // 4) % 512 < 24)
+        got = check(x, [7] * rows, 5)
+        assert ((got["top_ids"] % part // 4) % 512 < 24).all()
+    x = torch.full((3, 151936), -math.inf, device="cuda")
+    x[:, 77::50000] = torch.arange(12, device="cuda").float().reshape(3, 4)
+    got = check(x, [77, 78, 150077], 30)
+    assert np.array_equal(got["top_ids"][:, 4:], np.tile(np.r_[0:26], (3, 1)))
+
+
 def test_masked_and_non_finite_logits(cuda_lib, rng):
     """Masked tokens (-inf, the type's lowest value), NaN and +inf follow the sampler's rules; a row in which
     everything is masked is uniform."""
