@@ -298,18 +298,29 @@ def _row_stride(t) -> int:
     return t.stride(0) if t.shape[0] > 1 else 0
 
 
+def _ints(t, name: str, device, n: int | None = None) -> int:
+    """_check of a vector of int32 (of n entries), for calls made every step; returns its length."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1 and t.device == device
+            and t.is_contiguous() and (n is None or t.numel() == n)):
+        _check(t, name, torch.int32, (n,), device)
+    return t.numel()
+
+
 def _rows(kv, pos, row_seq, device):
-    rows = _check(pos, "pos", torch.int32, (None,), device).numel()
+    rows = _ints(pos, "pos", device)
     if row_seq is not None:
-        _check(row_seq, "row_seq", torch.int32, (rows,), device)
+        _ints(row_seq, "row_seq", device, rows)
     if rows < 1 or (row_seq is None and rows > kv.n_seqs):
         raise ValueError("one row per sequence without row_seq, and at least one")
     return rows
 
 
-def _on_current(device):
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"the tensors are on {device}, but cuda:{torch.cuda.current_device()} is the current device")
+def _stream_on(device) -> int:
+    """The current stream of the tensors' device, which must be the current one (launches go there)."""
+    i = torch.cuda.current_device()
+    if device.index != i:
+        raise ValueError(f"the tensors are on {device}, but cuda:{i} is the current device")
+    return torch._C._cuda_getCurrentRawStream(i)
 
 
 def paged_append_job(kv, layer: int, q, k, v, q_out, pos, rope_cs, row_seq=None, interleaved: bool = True):
@@ -337,8 +348,9 @@ def paged_append_job(kv, layer: int, q, k, v, q_out, pos, rope_cs, row_seq=None,
 
 def rope_kv_paged(job):
     """RoPE of the job's rows and their k and v into their pages (gsdlq_rope_kv_paged)."""
-    _on_current(job.device)
-    L.check(_lib().gsdlq_rope_kv_paged(ctypes.byref(job), stream_handle()), "gsdlq_rope_kv_paged")
+    status = _lib().gsdlq_rope_kv_paged(job, _stream_on(job.device))
+    if status:
+        L.check(status, "gsdlq_rope_kv_paged")
 
 
 def attention_paged_work(kv, rows: int, n_heads: int) -> torch.Tensor:
@@ -373,8 +385,9 @@ def paged_attn_job(kv, layer: int, q, out, pos, sm_scale: float, work, row_seq=N
 
 def attention_paged(job):
     """Attention of the job's rows over their sequences' pages (gsdlq_attention_paged)."""
-    _on_current(job.device)
-    L.check(_lib().gsdlq_attention_paged(ctypes.byref(job), stream_handle()), "gsdlq_attention_paged")
+    status = _lib().gsdlq_attention_paged(job, _stream_on(job.device))
+    if status:
+        L.check(status, "gsdlq_attention_paged")
 
 
 def logprobs_job(logits, ids=None, logprob=None, entropy=None, top_ids=None, top_logprobs=None,
@@ -414,5 +427,6 @@ def logprobs_job(logits, ids=None, logprob=None, entropy=None, top_ids=None, top
 
 def logprobs_rows(job):
     """Log probabilities, entropy and top alternatives of the job's rows (gsdlq_logprobs_rows)."""
-    _on_current(job.device)
-    L.check(_lib().gsdlq_logprobs_rows(ctypes.byref(job), stream_handle()), "gsdlq_logprobs_rows")
+    status = _lib().gsdlq_logprobs_rows(job, _stream_on(job.device))
+    if status:
+        L.check(status, "gsdlq_logprobs_rows")

@@ -8,7 +8,6 @@ and is captured as one CUDA graph.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -55,7 +54,7 @@ class PagedKV:
         ops._check(v, "v", k.dtype, tuple(k.shape), dev)
         ops._check(table, "table", torch.int32, (None, None), dev)
         ops._check(refs, "refs", torch.int32, (k.shape[1],), dev)
-        self.k, self.v, self.table, self.refs = k, v, table, refs
+        self.k, self.v, self.table, self.refs, self.device = k, v, table, refs, dev
         self.n_layers, self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = k.shape
         self.n_seqs, self.max_blocks = table.shape
         if min(k.shape) < 1 or min(table.shape) < 1:
@@ -69,6 +68,7 @@ class PagedKV:
         n = max(L.PAGED_MAX_SEQS, self.n_pages // 2 + 1)
         self.src, self.dst = torch.full((n,), -1, **i32), torch.full((n,), -1, **i32)
         self.counts = torch.zeros(4, **i32)
+        self._lists = tuple(t.data_ptr() for t in (self.src, self.dst, self.counts))
         self._to = torch.zeros(self.n_pages, **i32)
         self._desc = L.PagedKVDesc(k=k.data_ptr(), v=v.data_ptr(), kv_type=KV_TYPES[k.dtype], layers=self.n_layers,
                                    n_pages=self.n_pages, page_size=self.page_size, n_kv_heads=self.n_kv_heads,
@@ -78,32 +78,28 @@ class PagedKV:
     def desc(self) -> L.PagedKVDesc:
         return self._desc
 
-    @property
-    def device(self):
-        return self.k.device
-
     # ------------------------------------------------------------------ pages
     def fork(self, parent):
         """Sequence b takes over the pages of sequence parent[b], all at once; b itself: kept, -1: freed
         (gsdlq_pages_fork).  parent: int32 device tensor [n_seqs]."""
-        ops._check(parent, "parent", torch.int32, (self.n_seqs,), self.k.device)
-        ops._on_current(self.k.device)
-        L.check(L.load().gsdlq_pages_fork(ctypes.byref(self._desc), parent.data_ptr(), ops.stream_handle()),
-                "gsdlq_pages_fork")
+        ops._ints(parent, "parent", self.device, self.n_seqs)
+        status = L.load().gsdlq_pages_fork(self._desc, parent.data_ptr(), ops._stream_on(self.device))
+        if status:
+            L.check(status, "gsdlq_pages_fork")
 
     def reserve(self, pos, row_seq=None):
         """A page of its own for every row's position (gsdlq_pages_reserve), with the contents copied where the
         page was shared (gsdlq_pages_copy).  pos, row_seq: int32 device tensors [rows], as in attention.
         Afterwards counts holds (pages copied, rows that got no page, pages taken)."""
-        rows = ops._rows(self, pos, row_seq, self.k.device)
+        rows = ops._rows(self, pos, row_seq, self.device)
         if rows > L.PAGED_MAX_SEQS:
             raise ValueError(f"at most {L.PAGED_MAX_SEQS} rows")
-        ops._on_current(self.k.device)
-        lib, sh, d = L.load(), ops.stream_handle(), ctypes.byref(self._desc)
-        src, dst, counts = self.src.data_ptr(), self.dst.data_ptr(), self.counts.data_ptr()
-        L.check(lib.gsdlq_pages_reserve(d, None if row_seq is None else row_seq.data_ptr(), pos.data_ptr(), rows, src,
-                                        dst, rows, counts, sh), "gsdlq_pages_reserve")
-        L.check(lib.gsdlq_pages_copy(d, src, dst, counts, rows, sh), "gsdlq_pages_copy")
+        stream, (src, dst, counts) = ops._stream_on(self.device), self._lists
+        status = L.load().gsdlq_pages_reserve(self._desc, None if row_seq is None else row_seq.data_ptr(),
+                                              pos.data_ptr(), rows, src, dst, rows, counts, stream)
+        if status:
+            L.check(status, "gsdlq_pages_reserve")
+        self._copy(src, dst, counts, rows, stream)
 
     def compact(self, max_moves: int | None = None):
         """Move the pages in use to the front of the pool, the highest first, at most ``max_moves`` of them
@@ -112,23 +108,26 @@ class PagedKV:
         most = self.n_pages // 2 + 1 if max_moves is None else min(int(max_moves), self.n_pages // 2 + 1)
         if most < 1:
             raise ValueError("max_moves must be at least 1")
-        ops._on_current(self.k.device)
-        lib, sh, d = L.load(), ops.stream_handle(), ctypes.byref(self._desc)
-        src, dst, counts = self.src.data_ptr(), self.dst.data_ptr(), self.counts.data_ptr()
-        L.check(lib.gsdlq_pages_compact(d, src, dst, most, counts, self._to.data_ptr(), 4 * self.n_pages, sh),
-                "gsdlq_pages_compact")
-        L.check(lib.gsdlq_pages_copy(d, src, dst, counts, most, sh), "gsdlq_pages_copy")
+        stream, (src, dst, counts) = ops._stream_on(self.device), self._lists
+        status = L.load().gsdlq_pages_compact(self._desc, src, dst, most, counts, self._to.data_ptr(),
+                                              4 * self.n_pages, stream)
+        if status:
+            L.check(status, "gsdlq_pages_compact")
+        self._copy(src, dst, counts, most, stream)
 
     def copy_pages(self, src, dst, counts):
         """Copy page src[i] over page dst[i] in every layer, i < counts[0] (gsdlq_pages_copy): int32 device
         tensors.  A page must not be a destination twice, nor a source and a destination."""
-        n = ops._check(src, "src", torch.int32, (None,), self.k.device).numel()
-        ops._check(dst, "dst", torch.int32, (n,), self.k.device)
-        if ops._check(counts, "counts", torch.int32, (None,), self.k.device).numel() < 1 or n < 1:
+        n = ops._ints(src, "src", self.device)
+        ops._ints(dst, "dst", self.device, n)
+        if ops._ints(counts, "counts", self.device) < 1 or n < 1:
             raise ValueError("src, dst and counts must not be empty")
-        ops._on_current(self.k.device)
-        L.check(L.load().gsdlq_pages_copy(ctypes.byref(self._desc), src.data_ptr(), dst.data_ptr(), counts.data_ptr(),
-                                          n, ops.stream_handle()), "gsdlq_pages_copy")
+        self._copy(src.data_ptr(), dst.data_ptr(), counts.data_ptr(), n, ops._stream_on(self.device))
+
+    def _copy(self, src, dst, counts, n, stream):
+        status = L.load().gsdlq_pages_copy(self._desc, src, dst, counts, n, stream)
+        if status:
+            L.check(status, "gsdlq_pages_copy")
 
     def resized(self, n_pages: int) -> "PagedKV":
         """This cache in a pool of ``n_pages`` pages, larger or (after compact) smaller: a new pool with the pages'
