@@ -52,6 +52,13 @@ __device__ __forceinline__ float warp_max(float v) {
   return v;
 }
 
+// 2^x, relative error up to 2^-22; 0 below 2^-126
+__device__ __forceinline__ float ex2_ftz(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // Streaming 8-byte global load that does not allocate in L1 (weights are read once).
 __device__ __forceinline__ uint2 ldg_stream_u2(const void* p) {
   uint2 r;

@@ -54,11 +54,6 @@ struct LpShared {
   lp_key_t cand[LP_CAP];
 };
 
-__device__ __forceinline__ float lp_ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
 __device__ __forceinline__ float lp_clean(float x) {
   const uint32_t b = __float_as_uint(x);
   if ((b & 0x7fffffffu) >= 0x7f800000u) x = b == 0x7f800000u ? 100.f : -1e4f;
@@ -79,7 +74,7 @@ __device__ __forceinline__ float lp_below(float x) { return x - fmaf(fabsf(x), 9
 __device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b, float c) {
   const LpSums hi = a.m >= b.m ? a : b, lo = a.m >= b.m ? b : a;
   if (lo.m == -INFINITY) return hi;
-  const float d = fmaxf((lo.m - hi.m) * c, -200.f), f = lp_ex2(d);
+  const float d = fmaxf((lo.m - hi.m) * c, -200.f), f = ex2_ftz(d);
   return {hi.m, fmaf(f, lo.s + 1.f, hi.s), fmaf(f, fmaf(d, lo.s + 1.f, lo.t), hi.t)};
 }
 
@@ -114,7 +109,7 @@ __device__ __forceinline__ void lp_add(LpThread& T, float (&x)[N], int at, int v
       T.vecs = vecs;
     }
     if (top > T.a.m) {
-      const float f = lp_ex2(fmaxf((T.a.m - top) * c, -200.f)), d = fmaxf((T.a.m - top) * c, -200.f);
+      const float f = ex2_ftz(fmaxf((T.a.m - top) * c, -200.f)), d = fmaxf((T.a.m - top) * c, -200.f);
       T.a.t = f * fmaf(d, T.a.s, T.a.t);
       T.a.s *= f;
       bool placed = false;
@@ -130,7 +125,7 @@ __device__ __forceinline__ void lp_add(LpThread& T, float (&x)[N], int at, int v
   }
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    const float d = fmaxf((x[k] - T.a.m) * c, -200.f), e = lp_ex2(d);
+    const float d = fmaxf((x[k] - T.a.m) * c, -200.f), e = ex2_ftz(d);
     T.a.s += e;
     T.a.t = fmaf(e, d, T.a.t);
   }

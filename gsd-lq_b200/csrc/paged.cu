@@ -97,13 +97,17 @@ __global__ void __launch_bounds__(256) rope_kv_paged_kernel(const __grid_constan
 }
 
 // ---------------------------------------------------------------------------------------
-// Attention.  Work is cut into units of PA_TOK positions of one item -- a row and up to eight query heads of
-// one kv head -- and all units of the launch, row by row, item by item, are dealt to the CTAs in equal
-// contiguous runs, whatever the rows' lengths are (they are known on the device only).  Inside a CTA the
-// warps take the units of its run in turn, each through a ring of its own of K and V tiles (cp.async, no
-// CTA-wide barrier in the loop), with a running maximum and sum per head.  Where an item ends, the warps merge
-// through shared memory; an item that several CTAs share is joined by the CTA that arrives last, in the
-// order of the CTAs, so the result does not depend on who that is.
+// Attention.  An item is a row and up to eight query heads of one kv head; its positions are cut into units of
+// PA_TOK.  All units of the launch, row by row, item by item, are dealt to the CTAs in equal contiguous runs,
+// whatever the rows' lengths are (they are known on the device only); an item counts PA_ITEM units more, for what
+// it costs besides its positions.  A short item that lies whole inside a run is taken by one warp, the next one by
+// the next warp; of any other item the warps take the units in turn, and merge through shared memory where it
+// ends.  An item that several CTAs share is joined by the CTA that arrives last, in the order of the CTAs, so
+// that the result does not depend on who that is.
+//
+// A warp's tiles go through a ring of its own of three slots (cp.async, no CTA-wide barrier in the loop): K of a
+// unit, V of it, K of the next, ...; a slot is filled again as soon as its tile is used, so that two tiles are on
+// their way while one is worked on.
 //
 // Both products run on mma.m16n8k16 with the 16-bit cache values as they are, so K and V go from shared
 // memory to the matrix unit without a conversion.  q and the weights p are fp32 and enter as parts of 16 bits:
@@ -115,22 +119,23 @@ __global__ void __launch_bounds__(256) rope_kv_paged_kernel(const __grid_constan
 constexpr int PA_MAX_CTAS = 320;  // largest grid of an attention launch
 constexpr int PA_GROUP = 8;       // query heads of one kv head taken together
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
-constexpr int PA_STAGES = 3;
-constexpr int PA_TILE = 4096;     // bytes of a unit's K or V tile
+constexpr int PA_SLOTS = 3;
+constexpr int PA_ITEM = 1;        // units that an item counts besides its own
+constexpr int PA_SHORT = 8;       // units of an item that one warp may take
+
+constexpr int pa_tok(int hd) { return hd == 128 ? 32 : 64; }  // positions of a unit
 
 template <int HD>
 struct PagedAttnSmem {
-  uint8_t ring[PA_WARPS][PA_STAGES][2 * PA_TILE];
+  uint8_t ring[PA_WARPS][PA_SLOTS][pa_tok(HD) * HD * 2];
   union {
     float acc[PA_WARPS][PA_GROUP][HD];  // the warps' results of an item
     float f[PA_GROUP][PA_MAX_CTAS];     // factors of the CTAs' parts, once those are written
   };
   float m[PA_WARPS][PA_GROUP], l[PA_WARPS][PA_GROUP];
   float fl[PA_GROUP];
-  unsigned long long valid[PA_WARPS][PA_STAGES];
-  long long warp_sum[PA_WARPS];
-  long long base;
-  int row, last;
+  int warp_sum[PA_WARPS];
+  int row, base, last;
 };
 
 inline size_t attention_paged_counters(int rows, int n_heads, int n_kv) {
@@ -143,15 +148,16 @@ inline size_t attention_paged_work(int rows, int n_heads, int n_kv, int hd) {
 }
 
 template <bool BF16>
-__device__ __forceinline__ void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void pa_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                       const float (&c)[4]) {
   if constexpr (BF16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
   else
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ void pa_ldm(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -165,8 +171,8 @@ __device__ __forceinline__ void pa_ldm_trans(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
-__device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src, bool ok) {  // zeros where not ok
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+__device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src, int bytes) {  // 16, or 0: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
 // (x, y) as parts of 16 bits: fp16 hi + lo, bf16 hi + mid + lo
@@ -196,257 +202,341 @@ __device__ __forceinline__ uint32_t pa_at(int j, int c) {
   return (uint32_t)(j * (HD * 2) + ((c ^ x) << 4));
 }
 
-// a walk over the units of the launch: the row and the unit it begins with
+// a walk over a CTA's run, segment by segment: the part of an item that lies in it
 struct PagedWalk {
-  long long base;  // first unit of the row
-  int row, tiles;  // units per item of the row
-  PagedRow pr;
+  PagedRow pr, next;     // the row, and the one after it, read ahead
+  int row, tiles, item;  // tiles: units of each of the row's items
+  int v;                 // where the next item begins
+  int s, a, b;           // the item's first unit; the segment is its units a .. b - 1
+  int t, step;           // this warp's next unit of it, and how far apart they are
+  int n_short;
+  bool whole, is_short;
 };
 
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(PA_THREADS, 2)
-    attention_paged_kernel(const __grid_constant__ gsdlq_paged_attn_job_t J, int subs) {
-  constexpr int TOK = PA_TILE / (HD * 2);  // positions of a unit: 16, 32, 64
-  constexpr int CH = HD / 8;               // 16-byte chunks of a row
+    attention_paged_kernel(const __grid_constant__ gsdlq_paged_attn_job_t J, int subs, int page_shift) {
+  constexpr int TOK = pa_tok(HD);
+  constexpr int TILE = TOK * HD * 2;       // bytes of a tile
+  constexpr int CH = HD / 8;               // 16-byte chunks of a position
   constexpr int KS = HD / 16;              // k steps of the first product
-  constexpr int TPL = (TOK + 31) / 32;     // positions a lane looks up
+  constexpr int TPL = TOK / 32;            // positions a lane looks up
   constexpr float P_SHIFT = BF16 ? 0.f : 11.f;
+  typedef unsigned long long mask_t;       // a bit per position of a unit
+  constexpr mask_t FULL = TOK == 64 ? ~0ull : (1ull << (TOK & 63)) - 1ull;
   extern __shared__ __align__(16) uint8_t pa_smem[];
   PagedAttnSmem<HD>& S = *reinterpret_cast<PagedAttnSmem<HD>*>(pa_smem);
   const gsdlq_paged_kv_t& kv = J.kv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
   const int gq_all = J.n_heads / kv.n_kv_heads, items_row = kv.n_kv_heads * subs;
   const size_t kw = (size_t)kv.n_kv_heads * HD;
+  auto row_tiles = [&](int len) { return (len + TOK - 1) / TOK; };
+  auto row_units = [&](int len) { return len > 0 ? (row_tiles(len) + PA_ITEM) * items_row : 0; };
 
-  // the launch's units, this CTA's run of them, and the row where it begins
-  long long sum = 0;
-  for (int r = tid; r < J.rows; r += PA_THREADS)
-    sum += (paged_row(kv, J.row_seq, J.pos, r, cta == 0).len + TOK - 1) / TOK;
+  // ---- the launch's units, this CTA's run of them, and the row where it begins
+  int mine0 = 0, sum = 0;  // of this thread's first row; of all its rows
+  for (int r = tid; r < J.rows; r += PA_THREADS) {
+    const int n = row_units(paged_row(kv, J.row_seq, J.pos, r, cta == 0).len);
+    if (r == tid) mine0 = n;
+    sum += n;
+  }
+  auto scan = [&](int n, int& total) {  // exclusive, over the CTA
+    int inc = n;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  if (lane == 0) S.warp_sum[warp] = sum;
-  if (tid == 0) S.row = -1;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    __syncthreads();
+    if (lane == 31) S.warp_sum[warp] = inc;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) {
+      before += w < warp ? S.warp_sum[w] : 0;
+      total += S.warp_sum[w];
+    }
+    return before + inc - n;
+  };
+  int units;
+  const int base0 = scan(sum, units);  // with one row a thread, also where that row begins
+  const int per = max((units + (int)gridDim.x - 1) / (int)gridDim.x, PA_WARPS + PA_ITEM);
+  const long long v0l = (long long)per * cta;
+  const int v0 = v0l < units ? (int)v0l : units, v1 = min(v0 + per, units);
   for (int r = cta; r < J.rows; r += gridDim.x)  // idle rows
     if (paged_row(kv, J.row_seq, J.pos, r, false).len == 0)
       for (int i = tid; i < J.n_heads * HD; i += PA_THREADS) J.out[(size_t)r * J.n_heads * HD + i] = 0.f;
-  __syncthreads();
-  long long units = 0;
-#pragma unroll
-  for (int w = 0; w < PA_WARPS; ++w) units += S.warp_sum[w];
-  units *= items_row;
-  const long long per = max((units + gridDim.x - 1) / (long long)gridDim.x, (long long)PA_WARPS);
-  const long long u0 = per * cta, u1 = min(units, u0 + per);
-  if (u0 >= u1) return;
-  if (warp == 0) {  // find the row of u0
-    long long before = 0;
-    for (int r0 = 0; r0 < J.rows; r0 += 32) {
-      const int r = r0 + lane;
-      const long long n =
-          r < J.rows ? (long long)((paged_row(kv, J.row_seq, J.pos, r, false).len + TOK - 1) / TOK) * items_row : 0;
-      long long inc = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += u;
-      }
-      if (before + inc - n <= u0 && u0 < before + inc) {
+  if (v0 >= v1) return;
+  if (J.rows <= PA_THREADS) {
+    if (base0 <= v0 && v0 < base0 + mine0) {
+      S.row = tid;
+      S.base = base0;
+    }
+  } else {
+    int before = 0;
+    for (int r0 = 0; before <= v0; r0 += PA_THREADS) {  // (ends: v0 < units)
+      const int r = r0 + tid, n = r < J.rows ? row_units(paged_row(kv, J.row_seq, J.pos, r, false).len) : 0;
+      int total;
+      const int b = before + scan(n, total);
+      if (b <= v0 && v0 < b + n) {
         S.row = r;
-        S.base = before + inc - n;
+        S.base = b;
       }
-      before += __shfl_sync(0xffffffffu, inc, 31);
-      if (before > u0) break;
+      before += total;
     }
   }
   __syncthreads();
-  auto enter = [&](PagedWalk& w, int row, long long base) {
+
+  auto enter = [&](PagedWalk& w, int row) {  // w.next is the row's
     w.row = row;
-    w.base = base;
-    w.pr = paged_row(kv, J.row_seq, J.pos, row, false);
-    w.tiles = (w.pr.len + TOK - 1) / TOK;
+    w.pr = w.next;
+    w.tiles = row_tiles(w.pr.len);
+    if (row + 1 < J.rows) w.next = paged_row(kv, J.row_seq, J.pos, row + 1, false);
   };
-  auto advance = [&](PagedWalk& w, long long u) {  // to the row of unit u (u < units: it exists)
-    while (u >= w.base + (long long)w.tiles * items_row) enter(w, w.row + 1, w.base + (long long)w.tiles * items_row);
+  auto begin = [&](PagedWalk& w) {
+    w.next = paged_row(kv, J.row_seq, J.pos, S.row, false);
+    enter(w, S.row);
+    const int item = (v0 - S.base) / (w.tiles + PA_ITEM);
+    w.item = item - 1;
+    w.v = S.base + item * (w.tiles + PA_ITEM);
+    w.n_short = 0;
+    w.t = w.b = 0;
+  };
+  auto advance = [&](PagedWalk& w) {  // to the next segment; false: the run is at its end
+    do {
+      if (++w.item >= items_row) {
+        do {
+          if (w.row + 1 >= J.rows) return false;
+          enter(w, w.row + 1);
+        } while (w.tiles == 0);
+        w.item = 0;
+      }
+      w.s = w.v + PA_ITEM;
+      w.v = w.s + w.tiles;
+      if (w.s >= v1) return false;
+      w.a = max(v0 - w.s, 0);
+      w.b = min(v1 - w.s, w.tiles);
+    } while (w.a >= w.b);
+    w.whole = w.a == 0 && w.b == w.tiles;
+    // one warp for a short item only where there is work for the others
+    w.is_short = w.whole && w.tiles <= PA_SHORT && w.tiles * PA_WARPS <= v1 - v0;
+    w.step = w.is_short ? 1 : PA_WARPS;
+    w.t = !w.is_short ? w.a + warp : (w.n_short & (PA_WARPS - 1)) == warp ? w.a : w.b;
+    w.n_short += w.is_short;
+    return true;
   };
 
-  // ---- the ring: where a unit's rows are, one step before they are copied
+  // ---- the ring
   const uint16_t* const kp = static_cast<const uint16_t*>(kv.k) + (size_t)J.layer * kv.n_pages * kv.page_size * kw;
   const uint16_t* const vp = static_cast<const uint16_t*>(kv.v) + (size_t)J.layer * kv.n_pages * kv.page_size * kw;
   const uint32_t ring = smem_u32(S.ring[warp][0]);
+  struct Unit {            // where a unit's positions are
+    int page[TPL], at[TPL];  // page (-1: none), position in it, of position lane + 32 i
+    int head;                // kv head, -1: no unit
+  };
   PagedWalk ahead;
-  enter(ahead, S.row, S.base);
-  long long u_look = u0 + warp;  // next unit to look up
-  int at_page[TPL], at_slot[TPL], at_head;
-  auto look = [&]() {
-    at_head = -1;
-    if (u_look < u1) {
-      advance(ahead, u_look);
-      const int rel = (int)(u_look - ahead.base), item = rel / ahead.tiles, tile = rel - item * ahead.tiles;
-      at_head = item / subs;
+  bool more = true;
+  begin(ahead);
+  auto look = [&](Unit& U) {
+    U.head = -1;
 #pragma unroll
-      for (int i = 0; i < TPL; ++i) {
-        const int t = tile * TOK + i * 32 + lane;
-        at_page[i] = -1;
-        at_slot[i] = 0;
-        if ((TOK >= 32 || lane < TOK) && t < ahead.pr.len) {
-          const int b = t / kv.page_size;
-          at_slot[i] = t - b * kv.page_size;
-          at_page[i] = kv.table[(size_t)ahead.pr.seq * kv.max_blocks + b];
-          if (!paged_valid(kv, at_page[i])) raise_flag(GSDLQ_FLAG_BAD_PAGE);
-        }
+    for (int i = 0; i < TPL; ++i) U.page[i] = -1;
+    while (more && ahead.t >= ahead.b) more = advance(ahead);
+    if (!more) return;
+    U.head = subs == 1 ? ahead.item : ahead.item / subs;
+#pragma unroll
+    for (int i = 0; i < TPL; ++i) {
+      const int t = ahead.t * TOK + i * 32 + lane;
+      if (t < ahead.pr.len) {
+        const int b = page_shift >= 0 ? t >> page_shift : t / kv.page_size;
+        U.at[i] = t - b * kv.page_size;
+        U.page[i] = kv.table[(size_t)ahead.pr.seq * kv.max_blocks + b];
+        if (U.page[i] < 0) U.page[i] = kv.n_pages;  // missing: reported below
       }
     }
-    u_look += PA_WARPS;
+    ahead.t += ahead.step;
   };
-  auto copy = [&](int stage) {
-    if (at_head >= 0) {
-      long long off[TPL];
-      unsigned long long valid = 0;
+  // the unit's positions as places in the pool, -1: none
+  auto resolve = [&](const Unit& U, int (&slot)[TPL]) -> mask_t {
+    mask_t valid = 0;
 #pragma unroll
-      for (int i = 0; i < TPL; ++i) {
-        const bool ok = paged_valid(kv, at_page[i]);
-        off[i] = ok ? (long long)(((size_t)at_page[i] * kv.page_size + at_slot[i]) * kw + (size_t)at_head * HD) : -1;
-        valid |= (unsigned long long)__ballot_sync(0xffffffffu, ok) << (32 * i);
-      }
-      if (lane == 0) S.valid[warp][stage] = valid;
-      const uint32_t dst = ring + stage * 2 * PA_TILE;
+    for (int i = 0; i < TPL; ++i) {
+      const bool ok = paged_valid(kv, U.page[i]);
+      if (!ok && U.page[i] != -1) raise_flag(GSDLQ_FLAG_BAD_PAGE);
+      slot[i] = ok ? U.page[i] * kv.page_size + U.at[i] : -1;
+      valid |= (mask_t)__ballot_sync(0xffffffffu, ok) << (32 * i);
+    }
+    return valid;
+  };
+  auto copy = [&](const uint16_t* pool, int head, const int (&slot)[TPL], int to) {
+    if (head >= 0) {
+      const uint32_t dst = ring + to * TILE;
+      const char* const src = reinterpret_cast<const char*>(pool + (size_t)head * HD + (lane % CH) * 8);
 #pragma unroll
       for (int it = 0; it < TOK * CH / 32; ++it) {
-        const int e = it * 32 + lane, j = e / CH, c = e % CH;
-        const long long o = __shfl_sync(0xffffffffu, off[(it * 32 / CH) / 32], j & 31);
-        const size_t src = o < 0 ? 0 : (size_t)o + c * 8;
-        pa_cp16(dst + pa_at<HD>(j, c), kp + src, o >= 0);
-        pa_cp16(dst + PA_TILE + pa_at<HD>(j, c), vp + src, o >= 0);
+        const int j = it * (32 / CH) + lane / CH;
+        const int p = __shfl_sync(0xffffffffu, slot[it * (32 / CH) / 32], j & 31);
+        pa_cp16(dst + pa_at<HD>(j, lane % CH), src + (size_t)(unsigned)max(p, 0) * (kw * 2), p < 0 ? 0 : 16);
       }
     }
     cp_async_commit();
   };
-  look();
-#pragma unroll
-  for (int s = 0; s < PA_STAGES - 1; ++s) {
-    copy(s);
-    look();
-  }
 
-  // ---- item by item
+  // ---- queries of a segment, as loaded
+  PagedWalk cur;
+  begin(cur);
+  float2 x[KS][2];
+  auto seg_heads = [&](const PagedWalk& w, int& head0) {  // first query head, and how many
+    const int g = subs == 1 ? w.item : w.item / subs, sub = subs == 1 ? 0 : w.item - g * subs;
+    head0 = g * gq_all + sub * PA_GROUP;
+    return min(PA_GROUP, gq_all - sub * PA_GROUP);
+  };
+  auto next_seg = [&]() {  // to this warp's next segment, with its queries on their way
+    do {
+      if (!advance(cur)) return false;
+    } while (cur.is_short && cur.t >= cur.b);
+    int head0;
+    const int gq = seg_heads(cur, head0);
+    const float* q = J.q + cur.row * (J.q_stride ? (size_t)J.q_stride : (size_t)J.n_heads * HD) +
+                     (size_t)(head0 + min(lane >> 2, gq - 1)) * HD + 2 * (lane & 3);
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x[k][i] = *reinterpret_cast<const float2*>(q + k * 16 + i * 8);
+    return true;
+  };
+
+  // unit 0's K and V and unit 1's K on their way, unit 2 looked up
+  Unit U;
+  int slot[TPL], head;  // of the unit whose K is on its way and whose V is not
+  mask_t valid0, valid1;
+  {
+    Unit U0;
+    look(U0);
+    look(U);
+    valid0 = resolve(U0, slot);
+    copy(kp, U0.head, slot, 0);
+    copy(vp, U0.head, slot, 1);
+  }
+  valid1 = resolve(U, slot);
+  head = U.head;
+  copy(kp, head, slot, 2);
+  look(U);
+  bool have = next_seg();
+  int ks = 0;  // the slot of the current unit's K
+
   float* const part = reinterpret_cast<float*>(static_cast<uint8_t*>(J.work) +
                                                ((size_t)J.rows * items_row * sizeof(unsigned) + 15) / 16 * 16);
-  unsigned* const arrived = static_cast<unsigned*>(J.work);
-  PagedWalk cur;
-  enter(cur, S.row, S.base);
-  long long u = u0 + warp;  // this warp's next unit
-  int stage = 0;
-  for (long long item_u = u0; item_u < u1;) {
-    advance(cur, item_u);
-    const int item = (int)((item_u - cur.base) / cur.tiles);
-    const long long i0 = cur.base + (long long)item * cur.tiles, i1 = i0 + cur.tiles;  // the item's units
-    const long long end = min(i1, u1);
-    const int g = item / subs, sub = item - g * subs, gq = min(PA_GROUP, gq_all - sub * PA_GROUP);
-    const int head0 = g * gq_all + sub * PA_GROUP;
+  while (have) {
     // q of this lane's head as A fragments
     uint32_t qa[KS][4], ql[KS][2];
-    float s_scale;
+    float s_scale = J.sm_scale * 1.4426950408889634f;
     {
-      const int h = lane >> 2;
-      const float* q = J.q + cur.row * (J.q_stride ? (size_t)J.q_stride : (size_t)J.n_heads * HD) +
-                       (size_t)(head0 + min(h, gq - 1)) * HD + 2 * (lane & 3);
-      float2 x[KS][2];
-      float top = 0.f;
+      float up = 1.f, up2 = 1.f;
+      if (!BF16) {
+        // the largest entry to [2^14, 2^15), by a power of two; both factors stay normal numbers
+        float top = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) top = fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y)));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = top > 0.f && top < INFINITY ? min(max(14 - ilogbf(top), -114), 140) : 0;
+        up = __int_as_float((127 + e / 2) << 23);
+        up2 = __int_as_float((127 + e - e / 2) << 23);
+        s_scale *= __int_as_float((127 - e / 2) << 23) * __int_as_float((127 - (e - e / 2)) << 23);
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          x[k][i] = *reinterpret_cast<const float2*>(q + k * 16 + i * 8);
-          top = fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y)));
-        }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // fp16: the largest entry to [2^14, 2^15), by a power of two; both factors stay normal numbers
-      const int e = BF16 ? 0 : (top > 0.f && top < INFINITY) ? min(max(14 - ilogbf(top), -100), 140) : 0;
-      const float up = exp2f((float)(e / 2)), up2 = exp2f((float)(e - e / 2));
-      s_scale = J.sm_scale * 1.4426950408889634f;
-      if (!BF16) s_scale = s_scale / up / up2;
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t lo;
-          pa_split<BF16>(BF16 ? x[k][i].x : x[k][i].x * up * up2, BF16 ? x[k][i].y : x[k][i].y * up * up2, qa[k][2 * i],
-                         qa[k][2 * i + 1], lo);
-          ql[k][i] = lo;
-        }
+        for (int i = 0; i < 2; ++i)
+          pa_split<BF16>(x[k][i].x * up * up2, x[k][i].y * up * up2, qa[k][2 * i], qa[k][2 * i + 1], ql[k][i]);
     }
     float m = -INFINITY, l = 0.f, acc[CH][2];
 #pragma unroll
     for (int n = 0; n < CH; ++n) acc[n][0] = acc[n][1] = 0.f;
-    for (; u < end; u += PA_WARPS) {
-      int next = stage + PA_STAGES - 1;
-      next = next >= PA_STAGES ? next - PA_STAGES : next;
-      copy(next);
-      look();
-      asm volatile("cp.async.wait_group %0;" ::"n"(PA_STAGES - 1) : "memory");
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (; cur.t < cur.b; cur.t += cur.step) {
+      const uint32_t kt = ring + ks * TILE;
+      int vs = ks + 1;
+      vs = vs >= PA_SLOTS ? vs - PA_SLOTS : vs;
+      const uint32_t vt = ring + vs * TILE;
+      asm volatile("cp.async.wait_group %0;" ::"n"(PA_SLOTS - 1) : "memory");
       __syncwarp();
-      const uint32_t kt = ring + stage * 2 * PA_TILE, vt = kt + PA_TILE;
-      const unsigned long long valid = S.valid[warp][stage];
-      // scores of 8 positions a step
+      // scores, 8 positions a step
       float s[TOK / 8][4];
 #pragma unroll
-      for (int n = 0; n < TOK / 8; ++n) {
-        s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+      for (int k = 0; k < KS; k += 2) {
 #pragma unroll
-        for (int k = 0; k < KS; k += 2) {
+        for (int n = 0; n < TOK / 8; ++n) {
           uint32_t b[4];
           pa_ldm(b, kt + pa_at<HD>(n * 8 + (lane & 7), k * 2 + (lane >> 3)));
-          pa_mma<BF16>(s[n], qa[k], b[0], b[1]);
-          pa_mma<BF16>(s[n], qa[k + 1], b[2], b[3]);
+          if (k == 0)
+            pa_mma<BF16>(s[n], qa[k], b[0], b[1], zero);
+          else
+            pa_mma<BF16>(s[n], qa[k], b[0], b[1], s[n]);
+          pa_mma<BF16>(s[n], qa[k + 1], b[2], b[3], s[n]);
           if constexpr (BF16) {
             const uint32_t a0[4] = {ql[k][0], 0u, ql[k][1], 0u}, a1[4] = {ql[k + 1][0], 0u, ql[k + 1][1], 0u};
-            pa_mma<BF16>(s[n], a0, b[0], b[1]);
-            pa_mma<BF16>(s[n], a1, b[2], b[3]);
+            pa_mma<BF16>(s[n], a0, b[0], b[1], s[n]);
+            pa_mma<BF16>(s[n], a1, b[2], b[3], s[n]);
           }
         }
       }
+      __syncwarp();  // the K tile is read
+      copy(vp, head, slot, ks);
       // log2 weights, the running maximum
-      float top = -INFINITY;
-      float p[TOK / 8][2];
+      float top = -INFINITY, p[TOK / 8][2];
 #pragma unroll
       for (int n = 0; n < TOK / 8; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float x = (s[n][j] + s[n][j + 2]) * s_scale;
-          p[n][j] = (valid >> (n * 8 + 2 * (lane & 3) + j)) & 1ull ? x : -INFINITY;
-          top = fmaxf(top, p[n][j]);
-        }
+        for (int j = 0; j < 2; ++j) p[n][j] = (s[n][j] + s[n][j + 2]) * s_scale;
+      if (valid0 != FULL) {
+        const mask_t mine = valid0 >> (2 * (lane & 3));
+#pragma unroll
+        for (int n = 0; n < TOK / 8; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (!((mine >> (n * 8 + j)) & 1ull)) p[n][j] = -INFINITY;
+      }
+#pragma unroll
+      for (int n = 0; n < TOK / 8; ++n) top = fmaxf(top, fmaxf(p[n][0], p[n][1]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float mn = fmaxf(m, top);
-      const float ref = mn == -INFINITY ? 0.f : mn - P_SHIFT;
-      const float f = m == -INFINITY ? 0.f : exp2f(m - mn);
+      const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn, f = ex2_ftz(m - ref);
       m = mn;
-      l *= f;
       uint32_t pa[TOK / 16][4], pl[TOK / 16][2];
+      float ps = 0.f;
 #pragma unroll
       for (int n = 0; n < TOK / 8; ++n) {
-        p[n][0] = exp2f(p[n][0] - ref);
-        p[n][1] = exp2f(p[n][1] - ref);
-        l += p[n][0] + p[n][1];
-        uint32_t lo;
-        pa_split<BF16>(p[n][0], p[n][1], pa[n / 2][(n & 1) * 2], pa[n / 2][(n & 1) * 2 + 1], lo);
-        pl[n / 2][n & 1] = lo;
+        const float p0 = ex2_ftz(p[n][0] - (ref - P_SHIFT)), p1 = ex2_ftz(p[n][1] - (ref - P_SHIFT));
+        ps += p0 + p1;
+        pa_split<BF16>(p0, p1, pa[n / 2][(n & 1) * 2], pa[n / 2][(n & 1) * 2 + 1], pl[n / 2][n & 1]);
       }
+      l = fmaf(l, f, ps);
       // weighted values, 16 positions a step
+      asm volatile("cp.async.wait_group %0;" ::"n"(PA_SLOTS - 1) : "memory");
+      __syncwarp();
 #pragma unroll
       for (int n = 0; n < CH; n += 2) {
-        float o0[4] = {0.f, 0.f, 0.f, 0.f}, o1[4] = {0.f, 0.f, 0.f, 0.f};
+        float o0[4], o1[4];
 #pragma unroll
         for (int k = 0; k < TOK / 16; ++k) {
           uint32_t b[4];
           pa_ldm_trans(b, vt + pa_at<HD>(k * 16 + (lane & 15), n + (lane >> 4)));
-          pa_mma<BF16>(o0, pa[k], b[0], b[1]);
-          pa_mma<BF16>(o1, pa[k], b[2], b[3]);
+          if (k == 0) {
+            pa_mma<BF16>(o0, pa[k], b[0], b[1], zero);
+            pa_mma<BF16>(o1, pa[k], b[2], b[3], zero);
+          } else {
+            pa_mma<BF16>(o0, pa[k], b[0], b[1], o0);
+            pa_mma<BF16>(o1, pa[k], b[2], b[3], o1);
+          }
           if constexpr (BF16) {
             const uint32_t a[4] = {pl[k][0], 0u, pl[k][1], 0u};
-            pa_mma<BF16>(o0, a, b[0], b[1]);
-            pa_mma<BF16>(o1, a, b[2], b[3]);
+            pa_mma<BF16>(o0, a, b[0], b[1], o0);
+            pa_mma<BF16>(o1, a, b[2], b[3], o1);
           }
         }
         acc[n][0] = fmaf(acc[n][0], f, o0[0] + o0[2]);
@@ -454,93 +544,109 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
         acc[n + 1][0] = fmaf(acc[n + 1][0], f, o1[0] + o1[2]);
         acc[n + 1][1] = fmaf(acc[n + 1][1], f, o1[1] + o1[3]);
       }
-      __syncwarp();  // the tile is read
-      stage = stage + 1 == PA_STAGES ? 0 : stage + 1;
+      __syncwarp();  // the V tile is read
+      valid0 = valid1;
+      valid1 = resolve(U, slot);
+      head = U.head;
+      copy(kp, head, slot, vs);
+      look(U);
+      ks = ks + 2 >= PA_SLOTS ? ks + 2 - PA_SLOTS : ks + 2;
     }
-    // ---- the warps' results of the item
+    // ---- the segment's result
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    {
-      const int h = lane >> 2;
+    int head0;
+    const int gq = seg_heads(cur, head0), h = lane >> 2;
+    float* const out = J.out + ((size_t)cur.row * J.n_heads + head0) * HD;
+    auto inverse = [](float x) { return x > 0.f ? 1.f / x : (x == 0.f ? 0.f : NAN); };  // 0: no position left
+    if (cur.is_short) {  // all of the item, in this warp
       if (h < gq) {
+        const float inv = inverse(l);
 #pragma unroll
         for (int n = 0; n < CH; ++n)
-          *reinterpret_cast<float2*>(&S.acc[warp][h][n * 8 + 2 * (lane & 3)]) = make_float2(acc[n][0], acc[n][1]);
-        if ((lane & 3) == 0) {
-          S.m[warp][h] = m;
-          S.l[warp][h] = l;
-        }
+          *reinterpret_cast<float2*>(out + h * HD + n * 8 + 2 * (lane & 3)) = make_float2(acc[n][0] * inv, acc[n][1] * inv);
+      }
+      have = next_seg();
+      continue;
+    }
+    if (h < gq) {
+#pragma unroll
+      for (int n = 0; n < CH; ++n)
+        *reinterpret_cast<float2*>(&S.acc[warp][h][n * 8 + 2 * (lane & 3)]) = make_float2(acc[n][0], acc[n][1]);
+      if ((lane & 3) == 0) {
+        S.m[warp][h] = m;
+        S.l[warp][h] = l;
       }
     }
+    const bool whole = cur.whole;
+    const int first = cur.s / per, n_parts = (cur.s + cur.tiles - 1) / per - first + 1;  // CTAs that hold the item
+    float* const mine = part + ((size_t)cta * 2 + (cur.s >= v0)) * PA_GROUP * (HD + 2);
+    unsigned* const count = static_cast<unsigned*>(J.work) + (size_t)cur.row * items_row + cur.item;
+    have = next_seg();
     __syncthreads();
-    const bool whole = i0 >= u0 && i1 <= u1;
-    float* const mine = part + ((size_t)cta * 2 + (i0 >= u0)) * PA_GROUP * (HD + 2);
-    float* const out = J.out + ((size_t)cur.row * J.n_heads + head0) * HD;
     for (int e = tid; e < gq * HD; e += PA_THREADS) {
-      const int h = e / HD, d = e % HD;
-      float M = S.m[0][h];
+      const int hh = e / HD, d = e % HD;
+      float M = S.m[0][hh];
 #pragma unroll
-      for (int w = 1; w < PA_WARPS; ++w) M = fmaxf(M, S.m[w][h]);
+      for (int w = 1; w < PA_WARPS; ++w) M = fmaxf(M, S.m[w][hh]);
+      const float ref = M == -INFINITY ? 0.f : M;
       float L = 0.f, A = 0.f;
 #pragma unroll
       for (int w = 0; w < PA_WARPS; ++w) {
-        const float f = S.m[w][h] == -INFINITY ? 0.f : exp2f(S.m[w][h] - M);
-        L = fmaf(S.l[w][h], f, L);
-        A = fmaf(S.acc[w][h][d], f, A);
+        const float f = ex2_ftz(S.m[w][hh] - ref);
+        L = fmaf(S.l[w][hh], f, L);
+        A = fmaf(S.acc[w][hh][d], f, A);
       }
       if (whole) {
-        out[e] = L > 0.f ? A / L : (L == 0.f ? 0.f : NAN);
+        out[e] = A * inverse(L);
       } else {
         __stcg(mine + e, A);
         if (d == 0) {
-          __stcg(mine + PA_GROUP * HD + h, M);
-          __stcg(mine + PA_GROUP * (HD + 1) + h, L);
+          __stcg(mine + PA_GROUP * HD + hh, M);
+          __stcg(mine + PA_GROUP * (HD + 1) + hh, L);
         }
       }
     }
     if (!whole) {
-      // CTAs first .. last hold the item; its part lies in their second slot where it begins, else in the first
-      const int first = (int)(i0 / per), n_parts = (int)((i1 - 1) / per) - first + 1;
-      unsigned* const count = arrived + (size_t)cur.row * items_row + item;
+      // an item's part lies in its CTA's second place where it begins, else in the first
       __threadfence();
       __syncthreads();
       if (tid == 0) S.last = atomicAdd(count, 1u) == (unsigned)n_parts - 1u;
       __syncthreads();
       if (S.last) {
         __threadfence();
-        auto slot = [&](int i) { return part + ((size_t)(first + i) * 2 + (i == 0)) * PA_GROUP * (HD + 2); };
-        for (int h = warp; h < gq; h += PA_WARPS) {
+        auto place = [&](int i) { return part + ((size_t)(first + i) * 2 + (i == 0)) * PA_GROUP * (HD + 2); };
+        for (int hh = warp; hh < gq; hh += PA_WARPS) {
           float M = -INFINITY, L = 0.f;
           for (int i = lane; i < n_parts; i += 32) {
-            const float x = __ldcg(slot(i) + PA_GROUP * HD + h);
-            S.f[h][i] = x;
-            M = fmaxf(M, x);
+            const float z = __ldcg(place(i) + PA_GROUP * HD + hh);
+            S.f[hh][i] = z;
+            M = fmaxf(M, z);
           }
           M = warp_max(M);
+          const float ref = M == -INFINITY ? 0.f : M;
           for (int i = lane; i < n_parts; i += 32) {
-            const float f = S.f[h][i] == -INFINITY ? 0.f : exp2f(S.f[h][i] - M);
-            S.f[h][i] = f;
-            L = fmaf(__ldcg(slot(i) + PA_GROUP * (HD + 1) + h), f, L);
+            const float f = ex2_ftz(S.f[hh][i] - ref);
+            S.f[hh][i] = f;
+            L = fmaf(__ldcg(place(i) + PA_GROUP * (HD + 1) + hh), f, L);
           }
           L = warp_sum(L);
-          if (lane == 0) S.fl[h] = L;
+          if (lane == 0) S.fl[hh] = inverse(L);
         }
         __syncthreads();
         for (int e = tid; e < gq * HD; e += PA_THREADS) {
-          const int h = e / HD;
+          const int hh = e / HD;
           float A = 0.f;
 #pragma unroll 8
-          for (int i = 0; i < n_parts; ++i) A = fmaf(__ldcg(slot(i) + e), S.f[h][i], A);
-          const float L = S.fl[h];
-          out[e] = L > 0.f ? A / L : (L == 0.f ? 0.f : NAN);
+          for (int i = 0; i < n_parts; ++i) A = fmaf(__ldcg(place(i) + e), S.f[hh][i], A);
+          out[e] = A * S.fl[hh];
         }
         if (tid == 0) *count = 0u;
       }
     }
     __syncthreads();  // the merge area is free again
-    item_u = end;
   }
-  asm volatile("cp.async.wait_all;" ::: "memory");
+  cp_async_wait_all();
 }
 
 // ---------------------------------------------------------------------------------------
@@ -819,7 +925,8 @@ static int launch_attention_paged(const gsdlq_paged_attn_job_t& J, int subs, cud
     if (dev < 64) set[dev].store(true, std::memory_order_release);
   }
   const int grid = std::min(2 * num_sms(), PA_MAX_CTAS);
-  attention_paged_kernel<HD, BF16><<<grid, PA_THREADS, smem, st>>>(J, subs);
+  const int ps = J.kv.page_size, shift = ps & (ps - 1) ? -1 : __builtin_ctz((unsigned)ps);
+  attention_paged_kernel<HD, BF16><<<grid, PA_THREADS, smem, st>>>(J, subs, shift);
   GSDLQ_CUDA_CHECK_LAUNCH();
   return GSDLQ_OK;
 }
@@ -881,9 +988,9 @@ int gsdlq_attention_paged(const gsdlq_paged_attn_job_t* job, gsdlq_stream_t stre
   if (J.work_bytes < attention_paged_work(J.rows, J.n_heads, J.kv.n_kv_heads, J.kv.head_dim)) return GSDLQ_ERR_INVALID;
   const int gq = J.n_heads / J.kv.n_kv_heads, subs = (gq + PA_GROUP - 1) / PA_GROUP;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // a row's units are counted in 31 bits
-  const int tok = PA_TILE / (J.kv.head_dim * 2);
-  if (((long long)J.kv.max_blocks * J.kv.page_size / tok + 1) * J.kv.n_kv_heads * subs > INT32_MAX)
+  // units and places of a layer's pool are counted in 31 bits
+  const long long row_units = ((long long)J.kv.max_blocks * J.kv.page_size / pa_tok(J.kv.head_dim) + 2) * J.kv.n_kv_heads * subs;
+  if (row_units > INT32_MAX / 2 / J.rows || (long long)J.kv.n_pages * J.kv.page_size > INT32_MAX)
     return GSDLQ_ERR_UNSUPPORTED;
   switch (J.kv.head_dim * 2 + J.kv.kv_type) {
     case 32 * 2: return launch_attention_paged<32, false>(J, subs, st);
