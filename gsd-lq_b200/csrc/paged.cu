@@ -3,7 +3,9 @@
 // one contiguous cache (gsd_lq_cpu_engine.c:186-330); the per-row arithmetic is that of its functions.
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -105,9 +107,9 @@ __global__ void __launch_bounds__(256) rope_kv_paged_kernel(const __grid_constan
 // ends.  An item that several CTAs share is joined by the CTA that arrives last, in the order of the CTAs, so
 // that the result does not depend on who that is.
 //
-// A warp's tiles go through a ring of its own of three slots (cp.async, no CTA-wide barrier in the loop): K of a
-// unit, V of it, K of the next, ...; a slot is filled again as soon as its tile is used, so that two tiles are on
-// their way while one is worked on.
+// Each warp has a K and a V tile of its own (cp.async, no CTA-wide barrier in the loop): the next unit's K is on its
+// way while the weights and the second product are worked on, its V during the next first product.  Twelve such
+// warps an SM keep more bytes in flight and more instructions to choose from than eight with three tiles each.
 //
 // Both products run on mma.m16n8k16 with the 16-bit cache values as they are, so K and V go from shared
 // memory to the matrix unit without a conversion.  q and the weights p are fp32 and enter as parts of 16 bits:
@@ -116,10 +118,10 @@ __global__ void __launch_bounds__(256) rope_kv_paged_kernel(const __grid_constan
 // so that one product gives both parts and c[0] + c[2], c[1] + c[3] are the sums.  With A = q, B = K^T the score
 // fragment is already p's A fragment for the second product, B = V.  The second product starts from zero each
 // unit and is added to fp32 registers, which keeps the tensor core's truncating accumulation short.
-constexpr int PA_MAX_CTAS = 320;  // largest grid of an attention launch
+constexpr int PA_MAX_CTAS = 480;  // largest grid of an attention launch
+constexpr int PA_PER_SM = 2;
 constexpr int PA_GROUP = 8;       // query heads of one kv head taken together
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
-constexpr int PA_SLOTS = 3;
 constexpr int PA_ITEM = 1;        // units that an item counts besides its own
 constexpr int PA_SHORT = 8;       // units of an item that one warp may take
 
@@ -127,13 +129,9 @@ constexpr int pa_tok(int hd) { return hd == 128 ? 32 : 64; }  // positions of a 
 
 template <int HD>
 struct PagedAttnSmem {
-  uint8_t ring[PA_WARPS][PA_SLOTS][pa_tok(HD) * HD * 2];
-  union {
-    float acc[PA_WARPS][PA_GROUP][HD];  // the warps' results of an item
-    float f[PA_GROUP][PA_MAX_CTAS];     // factors of the CTAs' parts, once those are written
-  };
+  uint8_t tile[PA_WARPS][2][pa_tok(HD) * HD * 2];  // K, V
+  float acc[PA_WARPS][PA_GROUP][HD < 64 ? HD : 64];  // the warps' results of an item, 64 dimensions at a time
   float m[PA_WARPS][PA_GROUP], l[PA_WARPS][PA_GROUP];
-  float fl[PA_GROUP];
   int warp_sum[PA_WARPS];
   int row, base, last;
 };
@@ -171,6 +169,9 @@ __device__ __forceinline__ void pa_ldm_trans(uint32_t (&r)[4], uint32_t addr) {
                : "r"(addr)
                : "memory");
 }
+__device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void pa_cp16(uint32_t dst, const void* src, int bytes) {  // 16, or 0: zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
@@ -204,17 +205,16 @@ __device__ __forceinline__ uint32_t pa_at(int j, int c) {
 
 // a walk over a CTA's run, segment by segment: the part of an item that lies in it
 struct PagedWalk {
-  PagedRow pr, next;     // the row, and the one after it, read ahead
-  int row, tiles, item;  // tiles: units of each of the row's items
-  int v;                 // where the next item begins
-  int s, a, b;           // the item's first unit; the segment is its units a .. b - 1
-  int t, step;           // this warp's next unit of it, and how far apart they are
-  int n_short;
-  bool whole, is_short;
+  int row, seq, len, tiles;  // tiles: units of each of the row's items
+  int item, s;               // its first unit is the launch's unit s
+  int a, b;                  // the segment is its units a .. b - 1
+  int t, step;               // this warp's next unit of it, and how far apart they are
+  int n_short;               // short items so far
+  __device__ bool whole() const { return a == 0 && b == tiles; }
 };
 
 template <int HD, bool BF16>
-__global__ void __launch_bounds__(PA_THREADS, 2)
+__global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     attention_paged_kernel(const __grid_constant__ gsdlq_paged_attn_job_t J, int subs, int page_shift) {
   constexpr int TOK = pa_tok(HD);
   constexpr int TILE = TOK * HD * 2;       // bytes of a tile
@@ -222,12 +222,13 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
   constexpr int KS = HD / 16;              // k steps of the first product
   constexpr int TPL = TOK / 32;            // positions a lane looks up
   constexpr float P_SHIFT = BF16 ? 0.f : 11.f;
-  typedef unsigned long long mask_t;       // a bit per position of a unit
-  constexpr mask_t FULL = TOK == 64 ? ~0ull : (1ull << (TOK & 63)) - 1ull;
-  extern __shared__ __align__(16) uint8_t pa_smem[];
+  typedef typename std::conditional<TOK == 64, unsigned long long, unsigned>::type mask_t;  // a bit per position
+  constexpr mask_t FULL = ~(mask_t)0;
+  extern __shared__ __align__(1024) uint8_t pa_smem[];
   PagedAttnSmem<HD>& S = *reinterpret_cast<PagedAttnSmem<HD>*>(pa_smem);
   const gsdlq_paged_kv_t& kv = J.kv;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);  // (the same in all lanes, for the compiler to see)
   const int gq_all = J.n_heads / kv.n_kv_heads, items_row = kv.n_kv_heads * subs;
   const size_t kw = (size_t)kv.n_kv_heads * HD;
   auto row_tiles = [&](int len) { return (len + TOK - 1) / TOK; };
@@ -247,7 +248,6 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
       const int x = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += x;
     }
-    __syncthreads();
     if (lane == 31) S.warp_sum[warp] = inc;
     __syncthreads();
     int before = 0;
@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
     for (int r0 = 0; before <= v0; r0 += PA_THREADS) {  // (ends: v0 < units)
       const int r = r0 + tid, n = r < J.rows ? row_units(paged_row(kv, J.row_seq, J.pos, r, false).len) : 0;
       int total;
+      __syncthreads();  // the previous sums are read
       const int b = before + scan(n, total);
       if (b <= v0 && v0 < b + n) {
         S.row = r;
@@ -288,23 +289,23 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
   }
   __syncthreads();
 
-  auto enter = [&](PagedWalk& w, int row) {  // w.next is the row's
+  auto enter = [&](PagedWalk& w, int row) {
+    const PagedRow pr = paged_row(kv, J.row_seq, J.pos, row, false);
     w.row = row;
-    w.pr = w.next;
-    w.tiles = row_tiles(w.pr.len);
-    if (row + 1 < J.rows) w.next = paged_row(kv, J.row_seq, J.pos, row + 1, false);
+    w.seq = pr.seq;
+    w.len = pr.len;
+    w.tiles = row_tiles(pr.len);
   };
   auto begin = [&](PagedWalk& w) {
-    w.next = paged_row(kv, J.row_seq, J.pos, S.row, false);
     enter(w, S.row);
-    const int item = (v0 - S.base) / (w.tiles + PA_ITEM);
-    w.item = item - 1;
-    w.v = S.base + item * (w.tiles + PA_ITEM);
+    w.item = (v0 - S.base) / (w.tiles + PA_ITEM) - 1;  // the one before the run's first
+    w.s = S.base + w.item * (w.tiles + PA_ITEM) + PA_ITEM;
     w.n_short = 0;
     w.t = w.b = 0;
   };
   auto advance = [&](PagedWalk& w) {  // to the next segment; false: the run is at its end
     do {
+      w.s += w.tiles + PA_ITEM;
       if (++w.item >= items_row) {
         do {
           if (w.row + 1 >= J.rows) return false;
@@ -312,25 +313,23 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
         } while (w.tiles == 0);
         w.item = 0;
       }
-      w.s = w.v + PA_ITEM;
-      w.v = w.s + w.tiles;
       if (w.s >= v1) return false;
       w.a = max(v0 - w.s, 0);
       w.b = min(v1 - w.s, w.tiles);
     } while (w.a >= w.b);
-    w.whole = w.a == 0 && w.b == w.tiles;
     // one warp for a short item only where there is work for the others
-    w.is_short = w.whole && w.tiles <= PA_SHORT && w.tiles * PA_WARPS <= v1 - v0;
-    w.step = w.is_short ? 1 : PA_WARPS;
-    w.t = !w.is_short ? w.a + warp : (w.n_short & (PA_WARPS - 1)) == warp ? w.a : w.b;
-    w.n_short += w.is_short;
+    const bool is_short = w.whole() && w.tiles <= PA_SHORT && w.tiles * PA_WARPS <= v1 - v0;
+    w.step = is_short ? 1 : PA_WARPS;
+    w.t = !is_short ? w.a + warp : (w.n_short & (PA_WARPS - 1)) == warp ? w.a : w.b;
+    w.n_short += is_short;
     return true;
   };
 
-  // ---- the ring
+  // ---- the tiles
   const uint16_t* const kp = static_cast<const uint16_t*>(kv.k) + (size_t)J.layer * kv.n_pages * kv.page_size * kw;
   const uint16_t* const vp = static_cast<const uint16_t*>(kv.v) + (size_t)J.layer * kv.n_pages * kv.page_size * kw;
-  const uint32_t ring = smem_u32(S.ring[warp][0]);
+  const uint32_t row_bytes = (uint32_t)kw * 2;
+  const uint32_t kt = smem_u32(S.tile[warp][0]);
   struct Unit {            // where a unit's positions are
     int page[TPL], at[TPL];  // page (-1: none), position in it, of position lane + 32 i
     int head;                // kv head, -1: no unit
@@ -338,6 +337,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
   PagedWalk ahead;
   bool more = true;
   begin(ahead);
+  PagedWalk cur = ahead;
   auto look = [&](Unit& U) {
     U.head = -1;
 #pragma unroll
@@ -348,10 +348,10 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
 #pragma unroll
     for (int i = 0; i < TPL; ++i) {
       const int t = ahead.t * TOK + i * 32 + lane;
-      if (t < ahead.pr.len) {
+      if (t < ahead.len) {
         const int b = page_shift >= 0 ? t >> page_shift : t / kv.page_size;
         U.at[i] = t - b * kv.page_size;
-        U.page[i] = kv.table[(size_t)ahead.pr.seq * kv.max_blocks + b];
+        U.page[i] = kv.table[(size_t)ahead.seq * kv.max_blocks + b];
         if (U.page[i] < 0) U.page[i] = kv.n_pages;  // missing: reported below
       }
     }
@@ -369,23 +369,30 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
     }
     return valid;
   };
-  auto copy = [&](const uint16_t* pool, int head, const int (&slot)[TPL], int to) {
+  // chunk addresses differ by constants that are or-ed in below the tile's alignment: pa_at(j + 8 i, c) is
+  // pa_at(j, c) + 16 HD i, and pa_at(j, c ^ d) is pa_at(j, c) ^ 16 d
+  const uint32_t dst0 = kt + pa_at<HD>(lane / CH, lane % CH);
+  auto copy = [&](const uint16_t* pool, int head, const int (&slot)[TPL], mask_t valid, int to) {
     if (head >= 0) {
-      const uint32_t dst = ring + to * TILE;
       const char* const src = reinterpret_cast<const char*>(pool + (size_t)head * HD + (lane % CH) * 8);
+      const uint32_t dst = dst0 + to * TILE;
 #pragma unroll
       for (int it = 0; it < TOK * CH / 32; ++it) {
-        const int j = it * (32 / CH) + lane / CH;
-        const int p = __shfl_sync(0xffffffffu, slot[it * (32 / CH) / 32], j & 31);
-        pa_cp16(dst + pa_at<HD>(j, lane % CH), src + (size_t)(unsigned)max(p, 0) * (kw * 2), p < 0 ? 0 : 16);
+        constexpr int RI = 32 / CH;  // positions of a step; their bits of the position are below the lane's chunk's
+        const int j = it * RI;
+        const uint32_t x = CH >= 8 ? (uint32_t)((j & 7) << 4) : (uint32_t)(((j >> 1) & 3) << 4);
+        const int p = __shfl_sync(0xffffffffu, slot[j / 32], (j & 31) + lane / CH);
+        const uint32_t d = (dst ^ x) + j * (HD * 2);
+        if (valid == FULL)
+          pa_cp16(d, src + (size_t)(uint32_t)p * row_bytes);
+        else
+          pa_cp16(d, src + (size_t)(uint32_t)max(p, 0) * row_bytes, p < 0 ? 0 : 16);
       }
     }
     cp_async_commit();
   };
 
   // ---- queries of a segment, as loaded
-  PagedWalk cur;
-  begin(cur);
   float2 x[KS][2];
   auto seg_heads = [&](const PagedWalk& w, int& head0) {  // first query head, and how many
     const int g = subs == 1 ? w.item : w.item / subs, sub = subs == 1 ? 0 : w.item - g * subs;
@@ -395,7 +402,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
   auto next_seg = [&]() {  // to this warp's next segment, with its queries on their way
     do {
       if (!advance(cur)) return false;
-    } while (cur.is_short && cur.t >= cur.b);
+    } while (cur.step == 1 && cur.t >= cur.b);
     int head0;
     const int gq = seg_heads(cur, head0);
     const float* q = J.q + cur.row * (J.q_stride ? (size_t)J.q_stride : (size_t)J.n_heads * HD) +
@@ -407,35 +414,29 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
     return true;
   };
 
-  // unit 0's K and V and unit 1's K on their way, unit 2 looked up
+  // unit 0's K and V on their way, unit 1 looked up
   Unit U;
-  int slot[TPL], head;  // of the unit whose K is on its way and whose V is not
-  mask_t valid0, valid1;
-  {
-    Unit U0;
-    look(U0);
-    look(U);
-    valid0 = resolve(U0, slot);
-    copy(kp, U0.head, slot, 0);
-    copy(vp, U0.head, slot, 1);
-  }
-  valid1 = resolve(U, slot);
-  head = U.head;
-  copy(kp, head, slot, 2);
+  int slot[TPL], head;  // of the next unit
+  mask_t valid, valid_next;
+  look(U);
+  valid = resolve(U, slot);
+  copy(kp, U.head, slot, valid, 0);
+  copy(vp, U.head, slot, valid, 1);
   look(U);
   bool have = next_seg();
-  int ks = 0;  // the slot of the current unit's K
 
   float* const part = reinterpret_cast<float*>(static_cast<uint8_t*>(J.work) +
                                                ((size_t)J.rows * items_row * sizeof(unsigned) + 15) / 16 * 16);
+  // this lane's rows of the first K and V matrices
+  const uint32_t k0 = kt + pa_at<HD>(lane & 7, lane >> 3), vt0 = kt + TILE + pa_at<HD>(lane & 15, lane >> 4);
   while (have) {
     // q of this lane's head as A fragments
     uint32_t qa[KS][4], ql[KS][2];
     float s_scale = J.sm_scale * 1.4426950408889634f;
     {
-      float up = 1.f, up2 = 1.f;
+      float up = copysignf(1.f, s_scale);  // scores with the sign of the scale: the largest has the largest weight
       if (!BF16) {
-        // the largest entry to [2^14, 2^15), by a power of two; both factors stay normal numbers
+        // the largest entry to [2^14, 2^15), by a power of two (a row below 2^-112 not quite so far)
         float top = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k)
@@ -443,27 +444,23 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
           for (int i = 0; i < 2; ++i) top = fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y)));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = top > 0.f && top < INFINITY ? min(max(14 - ilogbf(top), -114), 140) : 0;
-        up = __int_as_float((127 + e / 2) << 23);
-        up2 = __int_as_float((127 + e - e / 2) << 23);
-        s_scale *= __int_as_float((127 - e / 2) << 23) * __int_as_float((127 - (e - e / 2)) << 23);
+        const int e = top > 0.f && top < INFINITY ? min(14 - ilogbf(top), 126) : 0;  // -113 .. 126
+        up *= __int_as_float((127 + e) << 23);
+        s_scale *= __int_as_float((127 - e) << 23);
       }
+      s_scale = fmaxf(fabsf(s_scale), FLT_MIN);  // (a masked position's -inf stays -inf)
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          pa_split<BF16>(x[k][i].x * up * up2, x[k][i].y * up * up2, qa[k][2 * i], qa[k][2 * i + 1], ql[k][i]);
+          pa_split<BF16>(x[k][i].x * up, x[k][i].y * up, qa[k][2 * i], qa[k][2 * i + 1], ql[k][i]);
     }
     float m = -INFINITY, l = 0.f, acc[CH][2];
 #pragma unroll
     for (int n = 0; n < CH; ++n) acc[n][0] = acc[n][1] = 0.f;
     const float zero[4] = {0.f, 0.f, 0.f, 0.f};
     for (; cur.t < cur.b; cur.t += cur.step) {
-      const uint32_t kt = ring + ks * TILE;
-      int vs = ks + 1;
-      vs = vs >= PA_SLOTS ? vs - PA_SLOTS : vs;
-      const uint32_t vt = ring + vs * TILE;
-      asm volatile("cp.async.wait_group %0;" ::"n"(PA_SLOTS - 1) : "memory");
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncwarp();
       // scores, 8 positions a step
       float s[TOK / 8][4];
@@ -472,7 +469,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
 #pragma unroll
         for (int n = 0; n < TOK / 8; ++n) {
           uint32_t b[4];
-          pa_ldm(b, kt + pa_at<HD>(n * 8 + (lane & 7), k * 2 + (lane >> 3)));
+          pa_ldm(b, (k0 ^ (k << 5)) + n * (HD * 16));
           if (k == 0)
             pa_mma<BF16>(s[n], qa[k], b[0], b[1], zero);
           else
@@ -486,38 +483,42 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
         }
       }
       __syncwarp();  // the K tile is read
-      copy(vp, head, slot, ks);
-      // log2 weights, the running maximum
+      valid_next = resolve(U, slot);
+      head = U.head;
+      copy(kp, head, slot, valid_next, 0);
+      // the scores, their maximum, the weights as powers of 2
       float top = -INFINITY, p[TOK / 8][2];
 #pragma unroll
       for (int n = 0; n < TOK / 8; ++n)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) p[n][j] = (s[n][j] + s[n][j + 2]) * s_scale;
-      if (valid0 != FULL) {
-        const mask_t mine = valid0 >> (2 * (lane & 3));
+        for (int j = 0; j < 2; ++j) p[n][j] = s[n][j] + s[n][j + 2];
+      if (valid != FULL) {
+        const mask_t mine = valid >> (2 * (lane & 3));
 #pragma unroll
         for (int n = 0; n < TOK / 8; ++n)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            if (!((mine >> (n * 8 + j)) & 1ull)) p[n][j] = -INFINITY;
+            if (!((mine >> (n * 8 + j)) & 1)) p[n][j] = -INFINITY;
       }
 #pragma unroll
       for (int n = 0; n < TOK / 8; ++n) top = fmaxf(top, fmaxf(p[n][0], p[n][1]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn, f = ex2_ftz(m - ref);
+      // m: the largest score so far, before the scale
+      const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn, f = ex2_ftz((m - ref) * s_scale);
+      const float shift = fmaf(-ref, s_scale, P_SHIFT);
       m = mn;
       uint32_t pa[TOK / 16][4], pl[TOK / 16][2];
       float ps = 0.f;
 #pragma unroll
       for (int n = 0; n < TOK / 8; ++n) {
-        const float p0 = ex2_ftz(p[n][0] - (ref - P_SHIFT)), p1 = ex2_ftz(p[n][1] - (ref - P_SHIFT));
+        const float p0 = ex2_ftz(fmaf(p[n][0], s_scale, shift)), p1 = ex2_ftz(fmaf(p[n][1], s_scale, shift));
         ps += p0 + p1;
         pa_split<BF16>(p0, p1, pa[n / 2][(n & 1) * 2], pa[n / 2][(n & 1) * 2 + 1], pl[n / 2][n & 1]);
       }
       l = fmaf(l, f, ps);
       // weighted values, 16 positions a step
-      asm volatile("cp.async.wait_group %0;" ::"n"(PA_SLOTS - 1) : "memory");
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncwarp();
 #pragma unroll
       for (int n = 0; n < CH; n += 2) {
@@ -525,7 +526,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
 #pragma unroll
         for (int k = 0; k < TOK / 16; ++k) {
           uint32_t b[4];
-          pa_ldm_trans(b, vt + pa_at<HD>(k * 16 + (lane & 15), n + (lane >> 4)));
+          pa_ldm_trans(b, (vt0 ^ (n << 4)) + k * (HD * 32));
           if (k == 0) {
             pa_mma<BF16>(o0, pa[k], b[0], b[1], zero);
             pa_mma<BF16>(o1, pa[k], b[2], b[3], zero);
@@ -545,12 +546,9 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
         acc[n + 1][1] = fmaf(acc[n + 1][1], f, o1[1] + o1[3]);
       }
       __syncwarp();  // the V tile is read
-      valid0 = valid1;
-      valid1 = resolve(U, slot);
-      head = U.head;
-      copy(kp, head, slot, vs);
+      copy(vp, head, slot, valid_next, 1);
+      valid = valid_next;
       look(U);
-      ks = ks + 2 >= PA_SLOTS ? ks + 2 - PA_SLOTS : ks + 2;
     }
     // ---- the segment's result
     l += __shfl_xor_sync(0xffffffffu, l, 1);
@@ -559,7 +557,7 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
     const int gq = seg_heads(cur, head0), h = lane >> 2;
     float* const out = J.out + ((size_t)cur.row * J.n_heads + head0) * HD;
     auto inverse = [](float x) { return x > 0.f ? 1.f / x : (x == 0.f ? 0.f : NAN); };  // 0: no position left
-    if (cur.is_short) {  // all of the item, in this warp
+    if (cur.step == 1) {  // all of the item, in this warp
       if (h < gq) {
         const float inv = inverse(l);
 #pragma unroll
@@ -569,41 +567,47 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
       have = next_seg();
       continue;
     }
-    if (h < gq) {
-#pragma unroll
-      for (int n = 0; n < CH; ++n)
-        *reinterpret_cast<float2*>(&S.acc[warp][h][n * 8 + 2 * (lane & 3)]) = make_float2(acc[n][0], acc[n][1]);
-      if ((lane & 3) == 0) {
-        S.m[warp][h] = m;
-        S.l[warp][h] = l;
-      }
-    }
-    const bool whole = cur.whole;
+    const bool whole = cur.whole();
     const int first = cur.s / per, n_parts = (cur.s + cur.tiles - 1) / per - first + 1;  // CTAs that hold the item
     float* const mine = part + ((size_t)cta * 2 + (cur.s >= v0)) * PA_GROUP * (HD + 2);
     unsigned* const count = static_cast<unsigned*>(J.work) + (size_t)cur.row * items_row + cur.item;
-    have = next_seg();
-    __syncthreads();
-    for (int e = tid; e < gq * HD; e += PA_THREADS) {
-      const int hh = e / HD, d = e % HD;
-      float M = S.m[0][hh];
+    constexpr int DIMS = HD < 64 ? HD : 64;
 #pragma unroll
-      for (int w = 1; w < PA_WARPS; ++w) M = fmaxf(M, S.m[w][hh]);
-      const float ref = M == -INFINITY ? 0.f : M;
-      float L = 0.f, A = 0.f;
+    for (int d0 = 0; d0 < HD; d0 += DIMS) {
+      if (d0 > 0) __syncthreads();  // the first dimensions are merged
+      if (h < gq) {
 #pragma unroll
-      for (int w = 0; w < PA_WARPS; ++w) {
-        const float f = ex2_ftz(S.m[w][hh] - ref);
-        L = fmaf(S.l[w][hh], f, L);
-        A = fmaf(S.acc[w][hh][d], f, A);
+        for (int n = 0; n < DIMS / 8; ++n)
+          *reinterpret_cast<float2*>(&S.acc[warp][h][n * 8 + 2 * (lane & 3)]) =
+              make_float2(acc[d0 / 8 + n][0], acc[d0 / 8 + n][1]);
+        if (d0 == 0 && (lane & 3) == 0) {
+          S.m[warp][h] = m * s_scale;
+          S.l[warp][h] = l;
+        }
       }
-      if (whole) {
-        out[e] = A * inverse(L);
-      } else {
-        __stcg(mine + e, A);
-        if (d == 0) {
-          __stcg(mine + PA_GROUP * HD + hh, M);
-          __stcg(mine + PA_GROUP * (HD + 1) + hh, L);
+      if (d0 + DIMS == HD) have = next_seg();
+      __syncthreads();
+      for (int e = tid; e < gq * DIMS / 4; e += PA_THREADS) {
+        const int hh = e / (DIMS / 4), d = e % (DIMS / 4) * 4;
+        float M = S.m[0][hh];
+#pragma unroll
+        for (int w = 1; w < PA_WARPS; ++w) M = fmaxf(M, S.m[w][hh]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        float L = 0.f;
+        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) {
+          const float f = ex2_ftz(S.m[w][hh] - ref);
+          const float4 o = *reinterpret_cast<const float4*>(&S.acc[w][hh][d]);
+          L = fmaf(S.l[w][hh], f, L);
+          A = make_float4(fmaf(o.x, f, A.x), fmaf(o.y, f, A.y), fmaf(o.z, f, A.z), fmaf(o.w, f, A.w));
+        }
+        if (whole) {
+          const float inv = inverse(L);
+          *reinterpret_cast<float4*>(out + hh * HD + d0 + d) = make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
+        } else {
+          __stcg(reinterpret_cast<float4*>(mine + hh * HD + d0 + d), A);
+          if (d0 + d == 0) __stcg(reinterpret_cast<float2*>(mine + PA_GROUP * HD) + hh, make_float2(M, L));
         }
       }
     }
@@ -615,31 +619,38 @@ __global__ void __launch_bounds__(PA_THREADS, 2)
       __syncthreads();
       if (S.last) {
         __threadfence();
-        auto place = [&](int i) { return part + ((size_t)(first + i) * 2 + (i == 0)) * PA_GROUP * (HD + 2); };
-        for (int hh = warp; hh < gq; hh += PA_WARPS) {
+        constexpr int BATCH = 8;  // parts whose loads are in flight together
+        for (int e = tid; e < gq * HD / 4; e += PA_THREADS) {
+          const int hh = e / (HD / 4);
           float M = -INFINITY, L = 0.f;
-          for (int i = lane; i < n_parts; i += 32) {
-            const float z = __ldcg(place(i) + PA_GROUP * HD + hh);
-            S.f[hh][i] = z;
-            M = fmaxf(M, z);
+          float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int i0 = 0; i0 < n_parts; i0 += BATCH) {
+            float4 o[BATCH];
+            float2 ml[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+              const int q = min(i0 + i, n_parts - 1);
+              const float* const at = part + ((size_t)(first + q) * 2 + (q == 0)) * PA_GROUP * (HD + 2);
+              o[i] = __ldcg(reinterpret_cast<const float4*>(at) + e);
+              ml[i] = __ldcg(reinterpret_cast<const float2*>(at + PA_GROUP * HD) + hh);
+              if (i0 + i >= n_parts) ml[i].x = -INFINITY;
+            }
+            float top = M;
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i].x);
+            const float ref = top == -INFINITY ? 0.f : top, f0 = ex2_ftz(M - ref);
+            M = top;
+            L *= f0;
+            A = make_float4(A.x * f0, A.y * f0, A.z * f0, A.w * f0);
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+              const float f = ex2_ftz(ml[i].x - ref);
+              L = fmaf(ml[i].y, f, L);
+              A = make_float4(fmaf(o[i].x, f, A.x), fmaf(o[i].y, f, A.y), fmaf(o[i].z, f, A.z), fmaf(o[i].w, f, A.w));
+            }
           }
-          M = warp_max(M);
-          const float ref = M == -INFINITY ? 0.f : M;
-          for (int i = lane; i < n_parts; i += 32) {
-            const float f = ex2_ftz(S.f[hh][i] - ref);
-            S.f[hh][i] = f;
-            L = fmaf(__ldcg(place(i) + PA_GROUP * (HD + 1) + hh), f, L);
-          }
-          L = warp_sum(L);
-          if (lane == 0) S.fl[hh] = inverse(L);
-        }
-        __syncthreads();
-        for (int e = tid; e < gq * HD; e += PA_THREADS) {
-          const int hh = e / HD;
-          float A = 0.f;
-#pragma unroll 8
-          for (int i = 0; i < n_parts; ++i) A = fmaf(__ldcg(place(i) + e), S.f[hh][i], A);
-          out[e] = A * S.fl[hh];
+          const float inv = inverse(L);
+          *(reinterpret_cast<float4*>(out) + e) = make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
         }
         if (tid == 0) *count = 0u;
       }
@@ -914,7 +925,7 @@ __global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(const __grid_c
 template <int HD, bool BF16>
 static int launch_attention_paged(const gsdlq_paged_attn_job_t& J, int subs, cudaStream_t st) {
   constexpr int smem = (int)sizeof(PagedAttnSmem<HD>);
-  static_assert(2 * (smem + 1024) <= 228 * 1024, "two CTAs an SM");
+  static_assert(PA_PER_SM * (smem + 1024) <= 228 * 1024, "shared memory of the CTAs of an SM");
   static std::atomic<bool> set[64];  // the opt-in shared memory size, once per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -924,7 +935,7 @@ static int launch_attention_paged(const gsdlq_paged_attn_job_t& J, int subs, cud
     if (e != cudaSuccess) return record_cuda_error(e);
     if (dev < 64) set[dev].store(true, std::memory_order_release);
   }
-  const int grid = std::min(2 * num_sms(), PA_MAX_CTAS);
+  const int grid = std::min(PA_PER_SM * num_sms(), PA_MAX_CTAS);
   const int ps = J.kv.page_size, shift = ps & (ps - 1) ? -1 : __builtin_ctz((unsigned)ps);
   attention_paged_kernel<HD, BF16><<<grid, PA_THREADS, smem, st>>>(J, subs, shift);
   GSDLQ_CUDA_CHECK_LAUNCH();
@@ -990,7 +1001,8 @@ int gsdlq_attention_paged(const gsdlq_paged_attn_job_t* job, gsdlq_stream_t stre
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // units and places of a layer's pool are counted in 31 bits
   const long long row_units = ((long long)J.kv.max_blocks * J.kv.page_size / pa_tok(J.kv.head_dim) + 2) * J.kv.n_kv_heads * subs;
-  if (row_units > INT32_MAX / 2 / J.rows || (long long)J.kv.n_pages * J.kv.page_size > INT32_MAX)
+  if (row_units > INT32_MAX / 2 / J.rows || (long long)J.kv.n_pages * J.kv.page_size > INT32_MAX ||
+      (long long)J.kv.n_kv_heads * J.kv.head_dim * 2 > INT32_MAX)
     return GSDLQ_ERR_UNSUPPORTED;
   switch (J.kv.head_dim * 2 + J.kv.kv_type) {
     case 32 * 2: return launch_attention_paged<32, false>(J, subs, st);
