@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(256) rope_kv_paged_kernel(const __grid_constan
 // ---------------------------------------------------------------------------------------
 // Attention.  An item is a row and up to eight query heads of one kv head; its positions are cut into units of
 // PA_TOK.  All units of the launch, row by row, item by item, are dealt to the CTAs in equal contiguous runs,
-// whatever the rows' lengths are (they are known on the device only); an item counts PA_ITEM units more, for what
+// whatever the rows' lengths are (they are known on the device only); an item counts some units more, for what
 // it costs besides its positions.  A short item that lies whole inside a run is taken by one warp, the next one by
 // the next warp; of any other item the warps take the units in turn, and merge through shared memory where it
 // ends.  An item that several CTAs share is joined by the CTA that arrives last, in the order of the CTAs, so
@@ -122,8 +122,9 @@ constexpr int PA_MAX_CTAS = 480;  // largest grid of an attention launch
 constexpr int PA_PER_SM = 2;
 constexpr int PA_GROUP = 8;       // query heads of one kv head taken together
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
-constexpr int PA_ITEM = 1;        // units that an item counts besides its own
-constexpr int PA_SHORT = 8;       // units of an item that one warp may take
+constexpr int PA_SHORT = 4;       // units of an item that one warp may take
+// units that an item counts besides its own, for its queries, and for the merge of the warps where it has one
+__host__ __device__ constexpr int pa_over(int tiles) { return tiles <= PA_SHORT ? 2 : 4; }
 
 constexpr int pa_tok(int hd) { return hd == 128 ? 32 : 64; }  // positions of a unit
 
@@ -209,7 +210,7 @@ struct PagedWalk {
   int item, s;               // its first unit is the launch's unit s
   int a, b;                  // the segment is its units a .. b - 1
   int t, step;               // this warp's next unit of it, and how far apart they are
-  int n_short;               // short items so far
+  unsigned long long load;   // what the warps have taken of short items, 16 bits each
   __device__ bool whole() const { return a == 0 && b == tiles; }
 };
 
@@ -232,7 +233,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
   const int gq_all = J.n_heads / kv.n_kv_heads, items_row = kv.n_kv_heads * subs;
   const size_t kw = (size_t)kv.n_kv_heads * HD;
   auto row_tiles = [&](int len) { return (len + TOK - 1) / TOK; };
-  auto row_units = [&](int len) { return len > 0 ? (row_tiles(len) + PA_ITEM) * items_row : 0; };
+  auto row_units = [&](int len) { return len > 0 ? (row_tiles(len) + pa_over(row_tiles(len))) * items_row : 0; };
 
   // ---- the launch's units, this CTA's run of them, and the row where it begins
   int mine0 = 0, sum = 0;  // of this thread's first row; of all its rows
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
   };
   int units;
   const int base0 = scan(sum, units);  // with one row a thread, also where that row begins
-  const int per = max((units + (int)gridDim.x - 1) / (int)gridDim.x, PA_WARPS + PA_ITEM);
+  const int per = max((units + (int)gridDim.x - 1) / (int)gridDim.x, PA_WARPS);
   const long long v0l = (long long)per * cta;
   const int v0 = v0l < units ? (int)v0l : units, v1 = min(v0 + per, units);
   for (int r = cta; r < J.rows; r += gridDim.x)  // idle rows
@@ -298,14 +299,15 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
   };
   auto begin = [&](PagedWalk& w) {
     enter(w, S.row);
-    w.item = (v0 - S.base) / (w.tiles + PA_ITEM) - 1;  // the one before the run's first
-    w.s = S.base + w.item * (w.tiles + PA_ITEM) + PA_ITEM;
-    w.n_short = 0;
+    const int n = w.tiles + pa_over(w.tiles);
+    w.item = (v0 - S.base) / n - 1;  // the one before the run's first
+    w.s = S.base + (w.item + 1) * n - w.tiles;
+    w.load = 0ull;
     w.t = w.b = 0;
   };
   auto advance = [&](PagedWalk& w) {  // to the next segment; false: the run is at its end
     do {
-      w.s += w.tiles + PA_ITEM;
+      const int end = w.s + w.tiles;
       if (++w.item >= items_row) {
         do {
           if (w.row + 1 >= J.rows) return false;
@@ -313,15 +315,30 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
         } while (w.tiles == 0);
         w.item = 0;
       }
+      w.s = end + pa_over(w.tiles);
       if (w.s >= v1) return false;
       w.a = max(v0 - w.s, 0);
       w.b = min(v1 - w.s, w.tiles);
     } while (w.a >= w.b);
-    // one warp for a short item only where there is work for the others
-    const bool is_short = w.whole() && w.tiles <= PA_SHORT && w.tiles * PA_WARPS <= v1 - v0;
+    // one warp for a short item, the one with the least so far; only where there is work for the others
+    const bool is_short = w.whole() && w.tiles <= PA_SHORT && w.tiles * 2 * PA_WARPS <= v1 - v0;
     w.step = is_short ? 1 : PA_WARPS;
-    w.t = !is_short ? w.a + warp : (w.n_short & (PA_WARPS - 1)) == warp ? w.a : w.b;
-    w.n_short += is_short;
+    w.t = w.a + warp;
+    if (is_short) {
+      int who = 0;
+      unsigned least = (unsigned)w.load & 0xffffu;
+#pragma unroll
+      for (int i = 1; i < PA_WARPS; ++i) {
+        const unsigned x = (unsigned)(w.load >> (16 * i)) & 0xffffu;
+        if (x < least) {
+          least = x;
+          who = i;
+        }
+      }
+      // (every warp comes to the same answer; a share past 16 bits would cost balance, nothing else)
+      w.load += (unsigned long long)(w.tiles + pa_over(w.tiles)) << (16 * who);
+      w.t = who == warp ? 0 : w.b;
+    }
     return true;
   };
 
@@ -1000,7 +1017,7 @@ int gsdlq_attention_paged(const gsdlq_paged_attn_job_t* job, gsdlq_stream_t stre
   const int gq = J.n_heads / J.kv.n_kv_heads, subs = (gq + PA_GROUP - 1) / PA_GROUP;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // units and places of a layer's pool are counted in 31 bits
-  const long long row_units = ((long long)J.kv.max_blocks * J.kv.page_size / pa_tok(J.kv.head_dim) + 2) * J.kv.n_kv_heads * subs;
+  const long long row_units = ((long long)J.kv.max_blocks * J.kv.page_size / pa_tok(J.kv.head_dim) + 8) * J.kv.n_kv_heads * subs;
   if (row_units > INT32_MAX / 2 / J.rows || (long long)J.kv.n_pages * J.kv.page_size > INT32_MAX ||
       (long long)J.kv.n_kv_heads * J.kv.head_dim * 2 > INT32_MAX)
     return GSDLQ_ERR_UNSUPPORTED;
