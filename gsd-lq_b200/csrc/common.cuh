@@ -192,6 +192,14 @@ __device__ __forceinline__ void named_bar_sync(int id, int threads) {
 __device__ __forceinline__ void named_bar_arrive(int id, int threads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+// ---- programmatic dependent launch --------------------------------------------------------------
+// A kernel launched by launch_pdl may be set up while the one before it on the stream still runs; it waits here
+// for that one's completion before it touches memory.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// From here on the next kernel may be set up.  Only kernels whose results no other kernel reads before its own
+// wait may say so early: not those that write the cache or its tables, which attention kernels read ahead.
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- thread-block clusters ---------------------------------------------------------------------
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -351,4 +359,26 @@ __device__ __forceinline__ unsigned long long argmax_key(float v, uint32_t idx) 
 namespace gsdlq {
 int record_cuda_error(cudaError_t e);
 int num_sms();
+
+// Launch with programmatic stream serialization, in clusters of `cluster` CTAs: the kernel must call pdl_wait()
+// before it reads or writes memory.
+template <typename... P, typename... A>
+int launch_pdl(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, unsigned cluster,
+               const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  return e == cudaSuccess ? GSDLQ_OK : record_cuda_error(e);
+}
 }  // namespace gsdlq

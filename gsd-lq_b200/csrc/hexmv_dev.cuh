@@ -362,8 +362,6 @@ __device__ __forceinline__ void wait_shared_flag(const volatile float* flag, int
   }
 }
 
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 struct StripInfo {
   int m0;     // matrix of the strip (the first of the pair in SwiGLU mode)

@@ -146,6 +146,8 @@ __device__ lp_key_t lp_block_max(LpShared& S, lp_key_t k) {
 __global__ void __launch_bounds__(LP_THREADS, 2)
     logprobs_rows_kernel(const __grid_constant__ gsdlq_logprobs_job_t J, int cluster) {
   __shared__ LpShared S;
+  pdl_wait();
+  pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r = blockIdx.x / cluster, rank = blockIdx.x - r * cluster;
   const float* const x = J.logits + (size_t)r * (J.row_stride ? J.row_stride : (size_t)J.n);
@@ -412,16 +414,6 @@ extern "C" int gsdlq_logprobs_rows(const gsdlq_logprobs_job_t* job, gsdlq_stream
   while (cluster < LP_MAX_CLUSTER && (long long)J.rows * cluster * 2 <= 2 * num_sms() && J.n / (cluster * 2) >= 2048)
     cluster *= 2;
   if ((long long)J.rows * cluster > INT32_MAX) return GSDLQ_ERR_INVALID;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(J.rows * cluster));
-  cfg.blockDim = dim3(LP_THREADS);
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logprobs_rows_kernel, J, cluster);
-  return e == cudaSuccess ? GSDLQ_OK : record_cuda_error(e);
+  return launch_pdl(logprobs_rows_kernel, (unsigned)(J.rows * cluster), LP_THREADS, 0, static_cast<cudaStream_t>(stream),
+                    (unsigned)cluster, J, cluster);
 }

@@ -51,6 +51,7 @@ __device__ __forceinline__ float kv_value(uint16_t b) {
 // RoPE + append.  One CTA per row.
 template <bool BF16>
 __global__ void __launch_bounds__(256) rope_kv_paged_kernel(const __grid_constant__ gsdlq_paged_append_job_t J) {
+  pdl_wait();
   const gsdlq_paged_kv_t& kv = J.kv;
   const int r = blockIdx.x, tid = threadIdx.x, hd = kv.head_dim, half = hd / 2;
   PagedRow row = paged_row(kv, J.row_seq, J.pos, r, tid == 0);
@@ -234,6 +235,9 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
   const size_t kw = (size_t)kv.n_kv_heads * HD;
   auto row_tiles = [&](int len) { return (len + TOK - 1) / TOK; };
   auto row_units = [&](int len) { return len > 0 ? (row_tiles(len) + pa_over(row_tiles(len))) * items_row : 0; };
+
+  pdl_wait();
+  pdl_launch_dependents();
 
   // ---- the launch's units, this CTA's run of them, and the row where it begins
   int mine0 = 0, sum = 0;  // of this thread's first row; of all its rows
@@ -683,6 +687,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
 __global__ void __launch_bounds__(256) pages_fork_kernel(const __grid_constant__ gsdlq_paged_kv_t kv,
                                                          const int* __restrict__ parent, int cols) {
   extern __shared__ int fork_tile[];  // [n_seqs][cols]
+  pdl_wait();
   const int c0 = blockIdx.x * cols, nc = min(cols, kv.max_blocks - c0);
   for (int e = threadIdx.x; e < kv.n_seqs * cols; e += blockDim.x) {
     const int b = e / cols, c = e - b * cols;
@@ -760,6 +765,7 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const __grid_
   __shared__ int page[GSDLQ_PAGED_MAX_SEQS], fresh[GSDLQ_PAGED_MAX_SEQS];
   __shared__ unsigned char dup[GSDLQ_PAGED_MAX_SEQS], failed[GSDLQ_PAGED_MAX_SEQS];
   __shared__ PageScan S;
+  pdl_wait();
   const int r = threadIdx.x;
   long long my_slot = -1;
   int my_page = -1;
@@ -847,6 +853,7 @@ __global__ void __launch_bounds__(PG_THREADS) pages_compact_kernel(const __grid_
                                                                    int* dst, int max_pairs, int* counts, int* to) {
   __shared__ PageScan S;
   __shared__ int high;
+  pdl_wait();
   const int tid = threadIdx.x;
   bool f[PG_PER];
   unsigned rank[PG_PER], live = 0, holes = 0;
@@ -895,6 +902,7 @@ __global__ void __launch_bounds__(PG_THREADS) pages_compact_kernel(const __grid_
 }
 __global__ void __launch_bounds__(256) pages_renumber_kernel(const __grid_constant__ gsdlq_paged_kv_t kv,
                                                              const int* __restrict__ to) {
+  pdl_wait();
   const size_t n = (size_t)kv.n_seqs * kv.max_blocks;
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
     const int p = kv.table[i];
@@ -909,6 +917,7 @@ __global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(const __grid_c
                                                                   const int* __restrict__ src,
                                                                   const int* __restrict__ dst,
                                                                   const int* __restrict__ counts, int max_pairs) {
+  pdl_wait();
   const int n = min(max(*counts, 0), max_pairs);
   const size_t words = (size_t)kv.page_size * kv.n_kv_heads * kv.head_dim / 8;  // of a page, one layer
   const size_t pieces = (words + COPY_PIECE - 1) / COPY_PIECE, per_pair = pieces * 2 * kv.layers;
@@ -954,9 +963,7 @@ static int launch_attention_paged(const gsdlq_paged_attn_job_t& J, int subs, cud
   }
   const int grid = std::min(PA_PER_SM * num_sms(), PA_MAX_CTAS);
   const int ps = J.kv.page_size, shift = ps & (ps - 1) ? -1 : __builtin_ctz((unsigned)ps);
-  attention_paged_kernel<HD, BF16><<<grid, PA_THREADS, smem, st>>>(J, subs, shift);
-  GSDLQ_CUDA_CHECK_LAUNCH();
-  return GSDLQ_OK;
+  return launch_pdl(attention_paged_kernel<HD, BF16>, grid, PA_THREADS, smem, st, 1, J, subs, shift);
 }
 
 static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -990,12 +997,8 @@ int gsdlq_rope_kv_paged(const gsdlq_paged_append_job_t* job, gsdlq_stream_t stre
     return GSDLQ_ERR_INVALID;
   if (J.q == J.q_out && J.q_stride != J.q_out_stride) return GSDLQ_ERR_INVALID;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (J.kv.kv_type == GSDLQ_KV_BF16)
-    rope_kv_paged_kernel<true><<<J.rows, 256, 0, st>>>(J);
-  else
-    rope_kv_paged_kernel<false><<<J.rows, 256, 0, st>>>(J);
-  GSDLQ_CUDA_CHECK_LAUNCH();
-  return GSDLQ_OK;
+  return launch_pdl(J.kv.kv_type == GSDLQ_KV_BF16 ? rope_kv_paged_kernel<true> : rope_kv_paged_kernel<false>,
+                    (unsigned)J.rows, 256, 0, st, 1, J);
 }
 
 int gsdlq_attention_paged_work_size(int rows, int n_heads, int n_kv_heads, int head_dim, size_t* bytes) {
@@ -1036,20 +1039,16 @@ int gsdlq_pages_fork(const gsdlq_paged_kv_t* kv, const int* parent, gsdlq_stream
   // columns of a CTA: 32 (whole 128-byte lines) while the tile of all sequences fits 48 KB, else 8
   const int cols = kv->n_seqs <= 384 ? 32 : 8;
   const unsigned grid = ((unsigned)kv->max_blocks + cols - 1) / cols;
-  pages_fork_kernel<<<grid, 256, sizeof(int) * (size_t)kv->n_seqs * cols, static_cast<cudaStream_t>(stream)>>>(*kv, parent,
-                                                                                                          cols);
-  GSDLQ_CUDA_CHECK_LAUNCH();
-  return GSDLQ_OK;
+  return launch_pdl(pages_fork_kernel, grid, 256, sizeof(int) * (size_t)kv->n_seqs * cols,
+                    static_cast<cudaStream_t>(stream), 1, *kv, parent, cols);
 }
 
 int gsdlq_pages_reserve(const gsdlq_paged_kv_t* kv, const int* row_seq, const int* pos, int rows, int* src, int* dst,
                         int max_pairs, int* counts, gsdlq_stream_t stream) {
   if (!kv || !pages_ok(*kv) || !rows_ok(*kv, row_seq, pos, rows) || rows > GSDLQ_PAGED_MAX_SEQS) return GSDLQ_ERR_INVALID;
   if (!src || !dst || !counts || max_pairs < rows) return GSDLQ_ERR_INVALID;
-  pages_reserve_kernel<<<1, PG_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(*kv, row_seq, pos, rows, src, dst,
-                                                                               max_pairs, counts);
-  GSDLQ_CUDA_CHECK_LAUNCH();
-  return GSDLQ_OK;
+  return launch_pdl(pages_reserve_kernel, 1, PG_THREADS, 0, static_cast<cudaStream_t>(stream), 1, *kv, row_seq, pos,
+                    rows, src, dst, max_pairs, counts);
 }
 
 int gsdlq_pages_compact(const gsdlq_paged_kv_t* kv, int* src, int* dst, int max_pairs, int* counts, void* work,
@@ -1057,21 +1056,19 @@ int gsdlq_pages_compact(const gsdlq_paged_kv_t* kv, int* src, int* dst, int max_
   if (!kv || !pages_ok(*kv) || !src || !dst || !counts || max_pairs <= 0 || !work) return GSDLQ_ERR_INVALID;
   if ((reinterpret_cast<uintptr_t>(work) & 3u) || work_bytes < sizeof(int) * (size_t)kv->n_pages) return GSDLQ_ERR_INVALID;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  pages_compact_kernel<<<1, PG_THREADS, 0, st>>>(*kv, src, dst, max_pairs, counts, static_cast<int*>(work));
-  GSDLQ_CUDA_CHECK_LAUNCH();
+  const int status = launch_pdl(pages_compact_kernel, 1, PG_THREADS, 0, st, 1, *kv, src, dst, max_pairs, counts,
+                                static_cast<int*>(work));
+  if (status != GSDLQ_OK) return status;
   const size_t n = (size_t)kv->n_seqs * kv->max_blocks;
-  pages_renumber_kernel<<<(unsigned)std::min<size_t>((n + 255) / 256, 1184), 256, 0, st>>>(*kv, static_cast<int*>(work));
-  GSDLQ_CUDA_CHECK_LAUNCH();
-  return GSDLQ_OK;
+  return launch_pdl(pages_renumber_kernel, (unsigned)std::min<size_t>((n + 255) / 256, 1184), 256, 0, st, 1, *kv,
+                    static_cast<const int*>(work));
 }
 
 int gsdlq_pages_copy(const gsdlq_paged_kv_t* kv, const int* src, const int* dst, const int* counts, int max_pairs,
                      gsdlq_stream_t stream) {
   if (!kv || !pool_ok(*kv) || !src || !dst || !counts || max_pairs <= 0) return GSDLQ_ERR_INVALID;
-  pages_copy_kernel<<<num_sms() * 8, COPY_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(*kv, src, dst, counts,
-                                                                                          max_pairs);
-  GSDLQ_CUDA_CHECK_LAUNCH();
-  return GSDLQ_OK;
+  return launch_pdl(pages_copy_kernel, (unsigned)(num_sms() * 8), COPY_THREADS, 0, static_cast<cudaStream_t>(stream), 1,
+                    *kv, src, dst, counts, max_pairs);
 }
 
 }  // extern "C"
