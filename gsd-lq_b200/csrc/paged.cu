@@ -910,38 +910,55 @@ __global__ void __launch_bounds__(256) pages_renumber_kernel(const __grid_consta
   }
 }
 
-// Pages: copy.  The pairs' pages of all layers are cut into pieces of COPY_PIECE 16-byte words, dealt to the
-// CTAs in turn.
-constexpr int COPY_THREADS = 256, COPY_PER = 4, COPY_PIECE = COPY_THREADS * COPY_PER;
-__global__ void __launch_bounds__(COPY_THREADS) pages_copy_kernel(const __grid_constant__ gsdlq_paged_kv_t kv,
-                                                                  const int* __restrict__ src,
-                                                                  const int* __restrict__ dst,
-                                                                  const int* __restrict__ counts, int max_pairs) {
+// Pages: copy.  The planes (layer, K or V) of the pairs' pages are cut into pieces of at most COPY_PIECE 16-byte
+// words, dealt to the CTAs in turn; the next piece's pair is looked up while a piece is copied.
+constexpr int COPY_THREADS = 128, COPY_PER = 4, COPY_PIECE = COPY_THREADS * COPY_PER;
+constexpr int COPY_PER_SM = 16;
+struct CopyPlan {
+  unsigned words;                   // of a plane of a page
+  unsigned pieces, per_pair;        // of a plane; of a page
+  unsigned step_pair, step_piece;   // from a CTA's piece to its next one: pairs, and pieces of them
+};
+__global__ void __launch_bounds__(COPY_THREADS, COPY_PER_SM)
+    pages_copy_kernel(const __grid_constant__ gsdlq_paged_kv_t kv, const __grid_constant__ CopyPlan P,
+                      const int* __restrict__ src, const int* __restrict__ dst, const int* __restrict__ counts,
+                      int max_pairs) {
   pdl_wait();
   const int n = min(max(*counts, 0), max_pairs);
-  const size_t words = (size_t)kv.page_size * kv.n_kv_heads * kv.head_dim / 8;  // of a page, one layer
-  const size_t pieces = (words + COPY_PIECE - 1) / COPY_PIECE, per_pair = pieces * 2 * kv.layers;
-  for (size_t c = blockIdx.x; c < (size_t)n * per_pair; c += gridDim.x) {
-    const int i = (int)(c / per_pair);
-    const size_t u = c - (size_t)i * per_pair, plane = u / pieces, piece = u - plane * pieces;
-    const int a = src[i], b = dst[i];
-    if (!paged_valid(kv, a) || !paged_valid(kv, b)) {
-      if (threadIdx.x == 0) raise_flag(GSDLQ_FLAG_BAD_PAGE);
-      continue;
-    }
-    uint4* pool = reinterpret_cast<uint4*>(plane & 1 ? kv.v : kv.k) + (plane >> 1) * kv.n_pages * words;
-    const uint4* from = pool + a * words;
-    uint4* into = pool + b * words;
+  unsigned i = blockIdx.x / P.per_pair, u = blockIdx.x % P.per_pair;
+  int a = -1, b = -1;
+  if (i < (unsigned)n) {
+    a = src[i];
+    b = dst[i];
+  }
+  while (i < (unsigned)n) {
+    const unsigned plane = u / P.pieces, e0 = (u - plane * P.pieces) * COPY_PIECE + threadIdx.x;
+    const bool ok = paged_valid(kv, a) && paged_valid(kv, b);
     uint4 w[COPY_PER];
+    uint4* const pool = reinterpret_cast<uint4*>(plane & 1 ? kv.v : kv.k) + (size_t)(plane >> 1) * kv.n_pages * P.words;
+    if (ok) {
+      const uint4* const from = pool + (size_t)a * P.words;
 #pragma unroll
-    for (int k = 0; k < COPY_PER; ++k) {
-      const size_t e = piece * COPY_PIECE + k * COPY_THREADS + threadIdx.x;
-      if (e < words) w[k] = from[e];
+      for (int k = 0; k < COPY_PER; ++k)
+        if (e0 + k * COPY_THREADS < P.words) w[k] = __ldcs(from + e0 + k * COPY_THREADS);
+    } else if (threadIdx.x == 0) {
+      raise_flag(GSDLQ_FLAG_BAD_PAGE);
     }
+    uint4* const into = pool + (size_t)b * P.words;
+    i += P.step_pair;
+    u += P.step_piece;
+    if (u >= P.per_pair) {
+      u -= P.per_pair;
+      ++i;
+    }
+    if (i < (unsigned)n) {
+      a = src[i];
+      b = dst[i];
+    }
+    if (ok) {
 #pragma unroll
-    for (int k = 0; k < COPY_PER; ++k) {
-      const size_t e = piece * COPY_PIECE + k * COPY_THREADS + threadIdx.x;
-      if (e < words) into[e] = w[k];
+      for (int k = 0; k < COPY_PER; ++k)
+        if (e0 + k * COPY_THREADS < P.words) __stcs(into + e0 + k * COPY_THREADS, w[k]);
     }
   }
 }
@@ -1067,8 +1084,13 @@ int gsdlq_pages_compact(const gsdlq_paged_kv_t* kv, int* src, int* dst, int max_
 int gsdlq_pages_copy(const gsdlq_paged_kv_t* kv, const int* src, const int* dst, const int* counts, int max_pairs,
                      gsdlq_stream_t stream) {
   if (!kv || !pool_ok(*kv) || !src || !dst || !counts || max_pairs <= 0) return GSDLQ_ERR_INVALID;
-  return launch_pdl(pages_copy_kernel, (unsigned)(num_sms() * 8), COPY_THREADS, 0, static_cast<cudaStream_t>(stream), 1,
-                    *kv, src, dst, counts, max_pairs);
+  const unsigned long long words = (unsigned long long)kv->page_size * kv->n_kv_heads * kv->head_dim / 8;
+  const unsigned long long per_pair = (words + COPY_PIECE - 1) / COPY_PIECE * 2 * kv->layers;
+  if (words > UINT32_MAX / 2 || per_pair > INT32_MAX) return GSDLQ_ERR_UNSUPPORTED;
+  const unsigned grid = (unsigned)num_sms() * COPY_PER_SM, pp = (unsigned)per_pair;
+  const CopyPlan P = {(unsigned)words, (unsigned)((words + COPY_PIECE - 1) / COPY_PIECE), pp, grid / pp, grid % pp};
+  return launch_pdl(pages_copy_kernel, grid, COPY_THREADS, 0, static_cast<cudaStream_t>(stream), 1, *kv, P, src, dst,
+                    counts, max_pairs);
 }
 
 }  // extern "C"
