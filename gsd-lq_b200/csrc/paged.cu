@@ -682,75 +682,91 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
 }
 
 // ---------------------------------------------------------------------------------------
-// Pages: fork.  A CTA owns `cols` columns of the table: it reads them whole, then writes the entries that
-// change and moves their counts.  The counts are integers, so the order of the atomics does not show.
-__global__ void __launch_bounds__(256) pages_fork_kernel(const __grid_constant__ gsdlq_paged_kv_t kv,
-                                                         const int* __restrict__ parent, int cols) {
-  extern __shared__ int fork_tile[];  // [n_seqs][cols]
+// Pages: fork.  A CTA owns FORK_COLS columns of the table (whole 32-byte sectors): it reads them whole, then writes
+// the entries that change and moves their counts.  The counts are integers, so the order of the atomics does not
+// show.
+constexpr int FORK_COLS = 8, FORK_THREADS = 512, FORK_ROWS = FORK_THREADS / FORK_COLS;
+__global__ void __launch_bounds__(FORK_THREADS) pages_fork_kernel(const __grid_constant__ gsdlq_paged_kv_t kv,
+                                                                  const int* __restrict__ parent) {
+  __shared__ int tile[GSDLQ_PAGED_MAX_SEQS][FORK_COLS];
   pdl_wait();
-  const int c0 = blockIdx.x * cols, nc = min(cols, kv.max_blocks - c0);
-  for (int e = threadIdx.x; e < kv.n_seqs * cols; e += blockDim.x) {
-    const int b = e / cols, c = e - b * cols;
-    if (c < nc) fork_tile[e] = kv.table[(size_t)b * kv.max_blocks + c0 + c];
+  const int c = threadIdx.x % FORK_COLS, b0 = threadIdx.x / FORK_COLS, col = blockIdx.x * FORK_COLS + c;
+  constexpr int UN = 4;  // rows in flight
+  for (int b = b0; b < kv.n_seqs; b += UN * FORK_ROWS) {
+    int e[UN];
+#pragma unroll
+    for (int i = 0; i < UN; ++i)
+      if (b + i * FORK_ROWS < kv.n_seqs && col < kv.max_blocks)
+        e[i] = kv.table[(size_t)(b + i * FORK_ROWS) * kv.max_blocks + col];
+#pragma unroll
+    for (int i = 0; i < UN; ++i)
+      if (b + i * FORK_ROWS < kv.n_seqs && col < kv.max_blocks) tile[b + i * FORK_ROWS][c] = e[i];
   }
+  int p[UN];  // the first rows' parents, before the barrier
+#pragma unroll
+  for (int i = 0; i < UN; ++i) p[i] = b0 + i * FORK_ROWS < kv.n_seqs ? parent[b0 + i * FORK_ROWS] : 0;
   __syncthreads();
-  for (int e = threadIdx.x; e < kv.n_seqs * cols; e += blockDim.x) {
-    const int b = e / cols, c = e - b * cols;
-    if (c >= nc) continue;
-    const int p = parent[b];
-    if (p < -1 || p >= kv.n_seqs) {
-      if (c == 0) raise_flag(GSDLQ_FLAG_BAD_PAGE);
-      continue;
+  if (col >= kv.max_blocks) return;
+  for (int b = b0; b < kv.n_seqs; b += UN * FORK_ROWS) {
+#pragma unroll
+    for (int i = 0; i < UN; ++i) {
+      const int r = b + i * FORK_ROWS;
+      if (r >= kv.n_seqs) break;
+      const int from = b == b0 ? p[i] : parent[r];
+      if (from < -1 || from >= kv.n_seqs) {
+        if (col == 0) raise_flag(GSDLQ_FLAG_BAD_PAGE);
+        continue;
+      }
+      const int was = tile[r][c], now = from < 0 ? -1 : tile[from][c];
+      if (was == now) continue;
+      kv.table[(size_t)r * kv.max_blocks + col] = now;
+      if (paged_valid(kv, was)) atomicAdd(&kv.refs[was], -1);
+      if (paged_valid(kv, now)) atomicAdd(&kv.refs[now], 1);
     }
-    const int was = fork_tile[e], now = p < 0 ? -1 : fork_tile[p * cols + c];
-    if (was == now) continue;
-    kv.table[(size_t)b * kv.max_blocks + c0 + c] = now;
-    if (paged_valid(kv, was)) atomicAdd(&kv.refs[was], -1);
-    if (paged_valid(kv, now)) atomicAdd(&kv.refs[now], 1);
   }
 }
 
 // ---------------------------------------------------------------------------------------
-// Block-wide scans over the pages' counts, 1024 threads: PG_PER pages a thread and step, a warp's 32
-// consecutive pages as one ballot, and one warp's scan over the step's 32 * PG_PER ballots.
-constexpr int PG_THREADS = 1024, PG_PER = 4, PG_STEP = PG_THREADS * PG_PER;
-struct PageScan {
-  unsigned cnt[32 * PG_PER];
-  unsigned total;
-};
-// f[i]: whether page base + i * 1024 + tid is wanted; rank[i]: how many wanted pages of this step come before
-// it.  Returns the number of wanted pages of the step.
-__device__ __forceinline__ unsigned page_scan(PageScan& S, const bool (&f)[PG_PER], unsigned (&rank)[PG_PER]) {
+// Block-wide scans over the pages' counts, 1024 threads: PG_PER consecutive pages a thread and step.
+constexpr int PG_THREADS = 1024, PG_WARPS = PG_THREADS / 32, PG_PER = 16, PG_STEP = PG_THREADS * PG_PER;
+// Exclusive sum of n over the block's threads, and the total.  `turn` alternates between calls, so that one
+// barrier a call is enough.
+__device__ __forceinline__ unsigned page_sum(unsigned (&sums)[2][PG_WARPS], int& turn, unsigned n, unsigned& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  unsigned m[PG_PER];
-  __syncthreads();  // the previous step's counts are read
+  unsigned inc = n;
 #pragma unroll
-  for (int i = 0; i < PG_PER; ++i) {
-    m[i] = __ballot_sync(0xffffffffu, f[i]);
-    if (lane == 0) S.cnt[i * 32 + warp] = __popc(m[i]);
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned x = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += x;
   }
+  if (lane == 31) sums[turn][warp] = inc;
   __syncthreads();
-  if (warp == 0) {
-    unsigned v[PG_PER], sum = 0;
+  unsigned w = sums[turn][lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned x = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += x;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const unsigned before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  turn ^= 1;
+  return (warp > 0 ? before : 0u) + inc - n;
+}
+// the counts of pages base .. base + PG_PER - 1 (0 past the end: neither in use nor, by `in`, free)
+__device__ __forceinline__ void page_counts(const gsdlq_paged_kv_t& kv, int base, int (&r)[PG_PER], unsigned& in) {
+  if (base + PG_PER <= kv.n_pages && (reinterpret_cast<uintptr_t>(kv.refs) & 15u) == 0u) {
+#pragma unroll
+    for (int i = 0; i < PG_PER; i += 4) *reinterpret_cast<int4*>(r + i) = *reinterpret_cast<const int4*>(kv.refs + base + i);
+    in = (1u << PG_PER) - 1u;
+  } else {
+    in = 0u;
 #pragma unroll
     for (int i = 0; i < PG_PER; ++i) {
-      v[i] = sum;
-      sum += S.cnt[lane * PG_PER + i];
+      const bool ok = base + i < kv.n_pages;
+      r[i] = ok ? kv.refs[base + i] : 0;
+      in |= (unsigned)ok << i;
     }
-    unsigned inc = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const unsigned u = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += u;
-    }
-#pragma unroll
-    for (int i = 0; i < PG_PER; ++i) S.cnt[lane * PG_PER + i] = inc - sum + v[i];
-    if (lane == 31) S.total = inc;
   }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < PG_PER; ++i) rank[i] = S.cnt[i * 32 + warp] + __popc(m[i] & ((1u << lane) - 1u));
-  return S.total;
 }
 
 // Pages: reserve.  One CTA, thread r = row r.  The rows act in order, so a row that shares its page with
@@ -763,12 +779,16 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const __grid_
                                                                    int* dst, int max_pairs, int* counts) {
   __shared__ long long slot[GSDLQ_PAGED_MAX_SEQS];
   __shared__ int page[GSDLQ_PAGED_MAX_SEQS], fresh[GSDLQ_PAGED_MAX_SEQS];
-  __shared__ unsigned char dup[GSDLQ_PAGED_MAX_SEQS], failed[GSDLQ_PAGED_MAX_SEQS];
-  __shared__ PageScan S;
+  __shared__ bool failed[GSDLQ_PAGED_MAX_SEQS];
+  __shared__ unsigned sums[2][PG_WARPS];
   pdl_wait();
   const int r = threadIdx.x;
+  int turn = 0;
+  int c[PG_PER];  // the first pages' counts, on their way while the rows are looked up
+  unsigned in;
+  page_counts(kv, r * PG_PER, c, in);
   long long my_slot = -1;
-  int my_page = -1;
+  int my_page = -1, held = 0;
   if (r < rows) {
     const PagedRow row = paged_row(kv, row_seq, pos, r, true);
     if (row.len > 0) {
@@ -777,69 +797,69 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const __grid_
       if (!paged_valid(kv, my_page)) {
         if (my_page != -1) raise_flag(GSDLQ_FLAG_BAD_PAGE);
         my_page = -1;
+      } else {
+        held = kv.refs[my_page];
       }
     }
-    slot[r] = my_slot;
-    page[r] = my_page;
-    failed[r] = 0;
   }
-  __syncthreads();
-  bool again = false;
-  if (my_slot >= 0)
-    for (int i = 0; i < r; ++i) again |= slot[i] == my_slot;
-  if (r < rows) dup[r] = again;
-  __syncthreads();
-  const bool acts = my_slot >= 0 && !again;
-  int before = 0;
-  if (acts && my_page >= 0)
-    for (int i = 0; i < r; ++i) before += page[i] == my_page && slot[i] >= 0 && !dup[i];
-  const int held = acts && my_page >= 0 ? kv.refs[my_page] : 0;
-  const bool shared = held - before > 1;
-  const bool need = acts && (my_page < 0 || shared);
-  bool f[PG_PER] = {need, false, false, false};
-  unsigned rank[PG_PER];
-  const unsigned wanted = page_scan(S, f, rank);
-  const unsigned my_rank = rank[0];
-  // the lowest free pages
-  unsigned have = 0;
-  for (int base = 0; base < kv.n_pages && have < wanted; base += PG_STEP) {
-#pragma unroll
-    for (int i = 0; i < PG_PER; ++i) {
-      const int p = base + i * PG_THREADS + r;
-      f[i] = p < kv.n_pages && kv.refs[p] <= 0;
+  // rows that may need a page: those of rows with one of their own need nothing, whatever the others do
+  const bool open = my_slot >= 0 && (my_page < 0 || held > 1);
+  unsigned wanted = 0, have = 0, pairs = 0, mine = 0;
+  int short_of = 0;
+  if (__syncthreads_or(open)) {
+    if (r < rows) {
+      slot[r] = my_slot;
+      page[r] = -1;
+      failed[r] = false;
     }
-    const unsigned n = page_scan(S, f, rank);
+    __syncthreads();
+    bool acts = open;
+    if (row_seq != nullptr && open)  // (without it every row has a sequence of its own)
+#pragma unroll 8
+      for (int i = 0; i < r; ++i) acts = acts && slot[i] != my_slot;
+    if (acts) page[r] = my_page;  // shared pages only, and of rows that act
+    __syncthreads();
+    int before = 0;
+    if (acts && my_page >= 0)
+#pragma unroll 8
+      for (int i = 0; i < r; ++i) before += page[i] == my_page;
+    const bool need = acts && (my_page < 0 || held - before > 1);
+    mine = page_sum(sums, turn, need, wanted);
+    // the lowest free pages
+    for (int base = 0; base < kv.n_pages && have < wanted; base += PG_STEP) {
+      unsigned n;
+      if (base > 0) page_counts(kv, base + r * PG_PER, c, in);
 #pragma unroll
-    for (int i = 0; i < PG_PER; ++i)
-      if (f[i] && have + rank[i] < wanted) fresh[have + rank[i]] = base + i * PG_THREADS + r;
-    have += n;
-  }
-  __syncthreads();  // fresh[] is complete, and every count has been read
-  const bool got = need && my_rank < have;
-  f[0] = got && my_page >= 0;
-  f[1] = f[2] = f[3] = false;
-  const unsigned pairs = page_scan(S, f, rank);
-  if (got) {
-    const int p = fresh[my_rank];
-    kv.table[my_slot] = p;
-    kv.refs[p] = 1;
-    if (my_page >= 0) {
-      atomicAdd(&kv.refs[my_page], -1);
-      src[rank[0]] = my_page;
-      dst[rank[0]] = p;
+      for (int i = 0; i < PG_PER; ++i)
+        if (c[i] > 0) in &= ~(1u << i);
+      unsigned at = have + page_sum(sums, turn, __popc(in), n);
+      for (; in != 0u && at < wanted; in &= in - 1u) fresh[at++] = base + r * PG_PER + __ffs(in) - 1;
+      have += n;
+    }
+    __syncthreads();  // fresh[] is complete, and every count has been read
+    const bool got = need && mine < have, copies = got && my_page >= 0;
+    const unsigned at = page_sum(sums, turn, copies, pairs);
+    if (got) {
+      const int p = fresh[mine];
+      kv.table[my_slot] = p;
+      kv.refs[p] = 1;
+      if (copies) {
+        atomicAdd(&kv.refs[my_page], -1);
+        src[at] = my_page;
+        dst[at] = p;
+      }
+    }
+    if (have < wanted) {  // exhausted (uniform): the last holder of a page that an earlier row could not leave fails too
+      bool fails = need && !got;
+      if (r < rows) failed[r] = fails;
+      __syncthreads();
+      if (acts && !need && before > 0)
+        for (int i = 0; i < r; ++i) fails |= page[i] == my_page && failed[i];
+      if (fails) raise_flag(GSDLQ_FLAG_NO_PAGE);
+      short_of = __syncthreads_count(fails);
     }
   }
   for (int i = pairs + r; i < max_pairs; i += PG_THREADS) src[i] = dst[i] = -1;
-  int short_of = 0;
-  if (have < wanted) {  // exhausted (uniform): the last holder of a page that an earlier row could not leave fails too
-    bool fails = need && !got;
-    if (r < rows) failed[r] = fails;
-    __syncthreads();
-    if (acts && !need && my_page >= 0 && before > 0)
-      for (int i = 0; i < r; ++i) fails |= page[i] == my_page && failed[i];
-    if (fails) raise_flag(GSDLQ_FLAG_NO_PAGE);
-    short_of = __syncthreads_count(fails);
-  }
   if (r == 0) {
     counts[0] = (int)pairs;
     counts[1] = short_of;
@@ -848,44 +868,74 @@ __global__ void __launch_bounds__(PG_THREADS) pages_reserve_kernel(const __grid_
 }
 
 // Pages: compact.  One CTA plans: the number of pages in use, then the free pages below it in ascending
-// order against the pages in use at and above it in descending order; `to` maps old to new pages.
+// order against the pages in use at and above it in descending order; `to` maps old to new pages.  Which pages are
+// in use is kept as bits in shared memory (of pools up to PG_KEPT * PG_STEP pages).  A table of up to PG_TABLE
+// entries is rewritten by the same CTA, a larger one by pages_renumber_kernel.
+constexpr int PG_KEPT = 16, PG_TABLE = 8192;
+__device__ __forceinline__ void pages_renumber(const gsdlq_paged_kv_t& kv, const int* to, size_t i, size_t step) {
+  const size_t n = (size_t)kv.n_seqs * kv.max_blocks;
+  for (; i < n; i += step) {
+    const int p = kv.table[i];
+    if (paged_valid(kv, p)) {
+      const int q = to[p];
+      if (q != p) kv.table[i] = q;
+    }
+  }
+}
 __global__ void __launch_bounds__(PG_THREADS) pages_compact_kernel(const __grid_constant__ gsdlq_paged_kv_t kv, int* src,
                                                                    int* dst, int max_pairs, int* counts, int* to) {
-  __shared__ PageScan S;
+  __shared__ unsigned sums[2][PG_WARPS];
+  __shared__ unsigned short kept[PG_KEPT][PG_THREADS];
   __shared__ int high;
   pdl_wait();
-  const int tid = threadIdx.x;
-  bool f[PG_PER];
-  unsigned rank[PG_PER], live = 0, holes = 0;
+  const int tid = threadIdx.x, steps = (kv.n_pages + PG_STEP - 1) / PG_STEP;
+  int turn = 0;
   if (tid == 0) high = 0;
-  auto scan = [&](auto wanted, auto take) {
-    unsigned seen = 0;
-    for (int base = 0; base < kv.n_pages; base += PG_STEP) {
+  // pages base .. base + PG_PER - 1 of step k: in use, and in the pool
+  auto used = [&](int k, bool again, unsigned& in) -> unsigned {
+    const int base = (k * PG_THREADS + tid) * PG_PER, left = kv.n_pages - base;
+    in = left >= PG_PER ? (1u << PG_PER) - 1u : left > 0 ? (1u << left) - 1u : 0u;
+    if (again && k < PG_KEPT) return kept[k][tid];
+    int c[PG_PER];
+    unsigned ok, m = 0u;
+    page_counts(kv, base, c, ok);
 #pragma unroll
-      for (int i = 0; i < PG_PER; ++i) {
-        const int p = base + i * PG_THREADS + tid;
-        f[i] = p < kv.n_pages && wanted(p);
-      }
-      const unsigned n = page_scan(S, f, rank);
-#pragma unroll
-      for (int i = 0; i < PG_PER; ++i)
-        if (f[i]) take(base + i * PG_THREADS + tid, seen + rank[i]);
-      seen += n;
-    }
-    return seen;
+    for (int i = 0; i < PG_PER; ++i) m |= (unsigned)(c[i] > 0) << i;
+    if (k < PG_KEPT) kept[k][tid] = (unsigned short)m;
+    return m;
   };
-  live = scan([&](int p) { return to[p] = p, kv.refs[p] > 0; }, [](int, unsigned) {});
-  holes = scan([&](int p) { return p < (int)live && kv.refs[p] <= 0; },
-               [&](int p, unsigned i) {
-                 if (i < (unsigned)max_pairs) dst[i] = p;
-               });
+  unsigned live = 0, in, n;
+  for (int k = 0; k < steps; ++k) live += __popc(used(k, false, in));
+  for (int p = tid; p < kv.n_pages; p += PG_THREADS) to[p] = p;
+  page_sum(sums, turn, live, n);
+  live = n;
+  // free pages below `live`, and pages in use at and above it: as many of the one as of the other
+  unsigned holes = 0, tails = 0;
+  auto below = [&](int base) -> unsigned {  // those of base .. that lie below `live`
+    const int left = (int)live - base;
+    return left >= PG_PER ? (1u << PG_PER) - 1u : left > 0 ? (1u << left) - 1u : 0u;
+  };
+  for (int k = 0; k * PG_STEP < (int)live; ++k) {
+    const int base = (k * PG_THREADS + tid) * PG_PER;
+    unsigned m = ~used(k, true, in);
+    m &= in & below(base);
+    unsigned at = holes + page_sum(sums, turn, __popc(m), n);
+    for (; m != 0u && at < (unsigned)max_pairs; m &= m - 1u) dst[at++] = base + __ffs(m) - 1;
+    holes += n;
+  }
   const unsigned moves = min(holes, (unsigned)max_pairs);
-  scan([&](int p) { return p >= (int)live && kv.refs[p] > 0; },
-       [&](int p, unsigned t) {
-         const unsigned i = holes - 1u - t;  // as many pages are in use above as are free below
-         if (i < moves) src[i] = p;
-         if (i == moves) high = p + 1;
-       });
+  for (int k = (int)(live / PG_STEP); k < steps && holes > 0; ++k) {
+    const int base = (k * PG_THREADS + tid) * PG_PER;
+    unsigned m = used(k, true, in) & ~below(base);
+    unsigned t = tails + page_sum(sums, turn, __popc(m), n);
+    for (; m != 0u; m &= m - 1u, ++t) {
+      const unsigned i = holes - 1u - t;
+      const int p = base + __ffs(m) - 1;
+      if (i < moves) src[i] = p;
+      if (i == moves) high = p + 1;
+    }
+    tails += n;
+  }
   __syncthreads();
   for (unsigned i = tid; i < moves; i += PG_THREADS) {
     const int a = src[i], b = dst[i];
@@ -899,15 +949,14 @@ __global__ void __launch_bounds__(PG_THREADS) pages_compact_kernel(const __grid_
     counts[1] = (int)live;
     counts[2] = moves == holes ? (int)live : high;
   }
-}
-__global__ void __launch_bounds__(256) pages_renumber_kernel(const __grid_constant__ gsdlq_paged_kv_t kv,
-                                                             const int* __restrict__ to) {
-  pdl_wait();
-  const size_t n = (size_t)kv.n_seqs * kv.max_blocks;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
-    const int p = kv.table[i];
-    if (paged_valid(kv, p) && to[p] != p) kv.table[i] = to[p];
+  if ((long long)kv.n_seqs * kv.max_blocks <= PG_TABLE) {
+    __syncthreads();  // `to` is complete
+    pages_renumber(kv, to, tid, PG_THREADS);
   }
+}
+__global__ void __launch_bounds__(256) pages_renumber_kernel(const __grid_constant__ gsdlq_paged_kv_t kv, const int* to) {
+  pdl_wait();
+  pages_renumber(kv, to, (size_t)blockIdx.x * 256 + threadIdx.x, (size_t)gridDim.x * 256);
 }
 
 // Pages: copy.  The planes (layer, K or V) of the pairs' pages are cut into pieces of at most COPY_PIECE 16-byte
@@ -1053,11 +1102,8 @@ int gsdlq_attention_paged(const gsdlq_paged_attn_job_t* job, gsdlq_stream_t stre
 
 int gsdlq_pages_fork(const gsdlq_paged_kv_t* kv, const int* parent, gsdlq_stream_t stream) {
   if (!kv || !pages_ok(*kv) || !parent) return GSDLQ_ERR_INVALID;
-  // columns of a CTA: 32 (whole 128-byte lines) while the tile of all sequences fits 48 KB, else 8
-  const int cols = kv->n_seqs <= 384 ? 32 : 8;
-  const unsigned grid = ((unsigned)kv->max_blocks + cols - 1) / cols;
-  return launch_pdl(pages_fork_kernel, grid, 256, sizeof(int) * (size_t)kv->n_seqs * cols,
-                    static_cast<cudaStream_t>(stream), 1, *kv, parent, cols);
+  const unsigned grid = ((unsigned)kv->max_blocks + FORK_COLS - 1) / FORK_COLS;
+  return launch_pdl(pages_fork_kernel, grid, FORK_THREADS, 0, static_cast<cudaStream_t>(stream), 1, *kv, parent);
 }
 
 int gsdlq_pages_reserve(const gsdlq_paged_kv_t* kv, const int* row_seq, const int* pos, int rows, int* src, int* dst,
@@ -1077,6 +1123,7 @@ int gsdlq_pages_compact(const gsdlq_paged_kv_t* kv, int* src, int* dst, int max_
                                 static_cast<int*>(work));
   if (status != GSDLQ_OK) return status;
   const size_t n = (size_t)kv->n_seqs * kv->max_blocks;
+  if (n <= PG_TABLE) return GSDLQ_OK;
   return launch_pdl(pages_renumber_kernel, (unsigned)std::min<size_t>((n + 255) / 256, 1184), 256, 0, st, 1, *kv,
                     static_cast<const int*>(work));
 }
