@@ -42,61 +42,64 @@ template <bool BF16>
 __device__ __forceinline__ uint16_t kv_round(float v) {
   return BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : f2h(v);
 }
-template <bool BF16>
-__device__ __forceinline__ float kv_value(uint16_t b) {
-  return BF16 ? __uint_as_float((uint32_t)b << 16) : h2f(b);
-}
 
 // ---------------------------------------------------------------------------------------
-// RoPE + append.  One CTA per row.
+// RoPE + append.  A thread per pair of one of the row's heads: query heads, then key heads, then value heads.  The
+// chain of look-ups (position, then angle and page, then the page's count) bounds it, so no thread does more than
+// one pair, and q does not wait for the page.
+constexpr int RK_THREADS = 256;
 template <bool BF16>
-__global__ void __launch_bounds__(256) rope_kv_paged_kernel(const __grid_constant__ gsdlq_paged_append_job_t J) {
+__global__ void __launch_bounds__(RK_THREADS)
+    rope_kv_paged_kernel(const __grid_constant__ gsdlq_paged_append_job_t J, int parts, int half_shift) {
   pdl_wait();
   const gsdlq_paged_kv_t& kv = J.kv;
-  const int r = blockIdx.x, tid = threadIdx.x, hd = kv.head_dim, half = hd / 2;
-  PagedRow row = paged_row(kv, J.row_seq, J.pos, r, tid == 0);
+  const int r = blockIdx.x / parts, e = (blockIdx.x - r * parts) * RK_THREADS + threadIdx.x;
+  const int half = 1 << half_shift, hd = 2 * half, h = e >> half_shift, i = e & (half - 1);
+  if (h >= J.n_heads + 2 * kv.n_kv_heads) return;
+  PagedRow row = paged_row(kv, J.row_seq, J.pos, r, e == 0);
   if (row.len > J.max_pos) {
-    if (tid == 0) raise_flag(GSDLQ_FLAG_BAD_POS);
+    if (e == 0) raise_flag(GSDLQ_FLAG_BAD_POS);
     row.len = 0;
   }
   const int pos = row.len - 1;
-  const size_t qw = (size_t)J.n_heads * hd, kw = (size_t)kv.n_kv_heads * hd;
-  const float* q = J.q + r * (J.q_stride ? (size_t)J.q_stride : qw);
-  float* qo = J.q_out + r * (J.q_out_stride ? (size_t)J.q_out_stride : qw);
-  if (row.len == 0) {
-    if (q != qo)
-      for (size_t i = tid; i < qw; i += blockDim.x) qo[i] = q[i];
+  const int i0 = J.interleaved ? 2 * i : i, i1 = J.interleaved ? 2 * i + 1 : i + half;
+  const float2* const cs = reinterpret_cast<const float2*>(J.rope_cs) + (size_t)pos * half + i;
+  if (h < J.n_heads) {
+    const size_t qw = (size_t)J.n_heads * hd;
+    const float* const q = J.q + r * (J.q_stride ? (size_t)J.q_stride : qw) + (size_t)h * hd;
+    float* const out = J.q_out + r * (J.q_out_stride ? (size_t)J.q_out_stride : qw) + (size_t)h * hd;
+    float x = q[i0], y = q[i1];
+    if (row.len > 0) {
+      const float2 c = *cs;
+      const float a = x, b = y;
+      x = __fsub_rn(__fmul_rn(a, c.x), __fmul_rn(b, c.y));
+      y = __fadd_rn(__fmul_rn(a, c.y), __fmul_rn(b, c.x));
+    }
+    out[i0] = x;
+    out[i1] = y;
     return;
   }
-  const float2* cs = reinterpret_cast<const float2*>(J.rope_cs) + (size_t)pos * half;
-  for (int e = tid; e < J.n_heads * half; e += blockDim.x) {
-    const int h = e / half, i = e - h * half;
-    const int i0 = h * hd + (J.interleaved ? 2 * i : i), i1 = h * hd + (J.interleaved ? 2 * i + 1 : i + half);
-    const float a = q[i0], b = q[i1];
-    const float2 c = cs[i];
-    qo[i0] = __fsub_rn(__fmul_rn(a, c.x), __fmul_rn(b, c.y));
-    qo[i1] = __fadd_rn(__fmul_rn(a, c.y), __fmul_rn(b, c.x));
+  if (row.len == 0) return;
+  const bool is_v = h >= J.n_heads + kv.n_kv_heads;
+  const int g = h - J.n_heads - (is_v ? kv.n_kv_heads : 0);
+  const size_t kw = (size_t)kv.n_kv_heads * hd;
+  const float* const in = (is_v ? J.v : J.k) + r * (J.kv_stride ? (size_t)J.kv_stride : kw) + (size_t)g * hd;
+  float x = in[i0], y = in[i1];
+  if (!is_v) {
+    const float2 c = *cs;
+    const float a = x, b = y;
+    x = __fsub_rn(__fmul_rn(a, c.x), __fmul_rn(b, c.y));
+    y = __fadd_rn(__fmul_rn(a, c.y), __fmul_rn(b, c.x));
   }
-  const int page = kv.table[(size_t)row.seq * kv.max_blocks + pos / kv.page_size];
+  const int block = pos / kv.page_size, page = kv.table[(size_t)row.seq * kv.max_blocks + block];
   if (!paged_valid(kv, page) || kv.refs[page] != 1) {
-    if (tid == 0) raise_flag(GSDLQ_FLAG_BAD_PAGE);
+    if (i == 0 && g == 0) raise_flag(GSDLQ_FLAG_BAD_PAGE);
     return;
   }
-  const size_t at = (((size_t)J.layer * kv.n_pages + page) * kv.page_size + pos % kv.page_size) * kw;
-  uint16_t* kd = static_cast<uint16_t*>(kv.k) + at;
-  uint16_t* vd = static_cast<uint16_t*>(kv.v) + at;
-  const float* k = J.k + r * (J.kv_stride ? (size_t)J.kv_stride : kw);
-  const float* v = J.v + r * (J.kv_stride ? (size_t)J.kv_stride : kw);
-  for (int e = tid; e < kv.n_kv_heads * half; e += blockDim.x) {
-    const int h = e / half, i = e - h * half;
-    const int i0 = h * hd + (J.interleaved ? 2 * i : i), i1 = h * hd + (J.interleaved ? 2 * i + 1 : i + half);
-    const float a = k[i0], b = k[i1];
-    const float2 c = cs[i];
-    kd[i0] = kv_round<BF16>(__fsub_rn(__fmul_rn(a, c.x), __fmul_rn(b, c.y)));
-    kd[i1] = kv_round<BF16>(__fadd_rn(__fmul_rn(a, c.y), __fmul_rn(b, c.x)));
-    vd[i0] = kv_round<BF16>(v[i0]);
-    vd[i1] = kv_round<BF16>(v[i1]);
-  }
+  const size_t at = (((size_t)J.layer * kv.n_pages + page) * kv.page_size + (pos - block * kv.page_size)) * kw + (size_t)g * hd;
+  uint16_t* const to = static_cast<uint16_t*>(is_v ? kv.v : kv.k) + at;
+  to[i0] = kv_round<BF16>(x);
+  to[i1] = kv_round<BF16>(y);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1058,13 +1061,16 @@ int gsdlq_rope_kv_paged(const gsdlq_paged_append_job_t* job, gsdlq_stream_t stre
   if (!J.q || !J.k || !J.v || !J.q_out || !J.rope_cs || J.max_pos <= 0 || J.n_heads <= 0) return GSDLQ_ERR_INVALID;
   if (J.layer < 0 || J.layer >= J.kv.layers) return GSDLQ_ERR_INVALID;
   const long long qw = (long long)J.n_heads * J.kv.head_dim, kw = (long long)J.kv.n_kv_heads * J.kv.head_dim;
-  if (qw > INT32_MAX || kw > INT32_MAX) return GSDLQ_ERR_INVALID;
+  if (qw > INT32_MAX / 4 || kw > INT32_MAX / 4) return GSDLQ_ERR_INVALID;
   if ((J.q_stride && J.q_stride < qw) || (J.q_out_stride && J.q_out_stride < qw) || (J.kv_stride && J.kv_stride < kw))
     return GSDLQ_ERR_INVALID;
   if (J.q == J.q_out && J.q_stride != J.q_out_stride) return GSDLQ_ERR_INVALID;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int half_shift = J.kv.head_dim == 128 ? 6 : J.kv.head_dim == 64 ? 5 : 4;
+  const long long parts = ((qw + 2 * kw) / 2 + RK_THREADS - 1) / RK_THREADS;
+  if (J.rows * parts > INT32_MAX) return GSDLQ_ERR_UNSUPPORTED;
   return launch_pdl(J.kv.kv_type == GSDLQ_KV_BF16 ? rope_kv_paged_kernel<true> : rope_kv_paged_kernel<false>,
-                    (unsigned)J.rows, 256, 0, st, 1, J);
+                    (unsigned)(J.rows * parts), RK_THREADS, 0, st, 1, J, (int)parts, half_shift);
 }
 
 int gsdlq_attention_paged_work_size(int rows, int n_heads, int n_kv_heads, int head_dim, size_t* bytes) {
