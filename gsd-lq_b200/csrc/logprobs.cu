@@ -21,7 +21,7 @@ namespace gsdlq {
 // ex2 and two additions.  Logits come in batches, so that lanes with a new maximum diverge once per batch.  Partial results (m1 >= m2) join as
 //   d = (m2 - m1) / temperature,  f = e^d,  s = s1 + f (s2 + 1),  t = t1 + f (t2 + d (s2 + 1)).
 //
-// Alternatives without a second pass over the row: the maxima of the 64 groups of eight threads are ranked.  Every
+// Alternatives without a second pass over the row: the maxima of the 128 groups of four threads are ranked.  Every
 // token of the best k has a key of at least the k-th largest group maximum, K, since k tokens have; and it lies in
 // one of the k groups whose maximum is at least K.  Only those groups' tokens are looked at again (they are in the
 // L2 cache); those at or above K -- mostly a few more than k -- are collected and ranked by counting.  Keys are
@@ -29,7 +29,7 @@ namespace gsdlq {
 // the groups' indices are looked up only where the k-th maximum is shared by more groups than are wanted, as in
 // rows with fewer unmasked tokens than k.
 constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
-constexpr int LP_GROUPS = LP_THREADS / 8;      // >= GSDLQ_MAX_TOP
+constexpr int LP_LANES = 4, LP_GROUPS = LP_THREADS / LP_LANES;  // groups of neighbouring lanes; >= GSDLQ_MAX_TOP
 constexpr int LP_CAP = 1280;                   // tokens collected before the slow path takes over
 constexpr int LP_MAX_CLUSTER = 8;
 typedef unsigned long long lp_key_t;
@@ -40,15 +40,14 @@ struct LpSums {
 struct LpShared {
   LpSums sums[LP_WARPS];
   LpSums part;                  // this CTA's
-  int n_top;                    // entries of top: k, or fewer where the CTA's part is shorter
-  lp_key_t top[GSDLQ_MAX_TOP];  // this CTA's best, in order
-  uint32_t gz[LP_GROUPS], kz;  // the groups' maxima, and the k-th largest of them
+  lp_key_t top[GSDLQ_MAX_TOP];  // this CTA's best, in order, then zeros
+  alignas(16) uint32_t gz[LP_GROUPS];  // the groups' maxima
+  uint32_t kz;                 // the k-th largest of them
   int over;                    // how many of the groups that share it are wanted, where not all are
   lp_key_t group[LP_GROUPS];   // their keys then
   lp_key_t K, red[LP_WARPS];
   lp_key_t all[LP_MAX_CLUSTER][GSDLQ_MAX_TOP];
   LpSums parts[LP_MAX_CLUSTER];
-  int counts[LP_MAX_CLUSTER];
   int n_list, list[GSDLQ_MAX_TOP];  // the groups that hold the CTA's best
   int found;
   lp_key_t cand[LP_CAP];
@@ -197,8 +196,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
   if (J.top > 0) {
     uint32_t g = my_z;
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if ((lane & 7) == 0) S.gz[tid >> 3] = g;
+    for (int o = LP_LANES / 2; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (lane % LP_LANES == 0) S.gz[tid / LP_LANES] = g;
   }
   if (tid == 0) {
     S.kz = 0u;
@@ -217,21 +216,27 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
   // ---- the CTA's best J.top tokens
   if (J.top > 0) {
     const int k = min(J.top, hi - lo);
-    if (tid < LP_GROUPS) {
-      const uint32_t g = S.gz[tid];
-      int above = 0, same = 0, first = 0;
-#pragma unroll 16
-      for (int j = 0; j < LP_GROUPS; ++j) {
-        above += S.gz[j] > g;
-        same += S.gz[j] == g;
-        first += S.gz[j] == g && j < tid;
+    {
+      // a group's lanes count a quarter of the others each
+      const int grp = tid / LP_LANES;
+      const uint32_t g = S.gz[grp];
+      int above = 0, same = 0;
+#pragma unroll
+      for (int j = 0; j < LP_GROUPS / (4 * LP_LANES); ++j) {
+        const uint4 z = *reinterpret_cast<const uint4*>(S.gz + 4 * (j * LP_LANES + lane % LP_LANES));
+        above += (z.x > g) + (z.y > g) + (z.z > g) + (z.w > g);
+        same += (z.x == g) + (z.y == g) + (z.z == g) + (z.w == g);
       }
-      if (above < k && g != 0u) {
-        if (above + same > k) {  // more groups share this maximum than belong to the best k
-          if (first == 0) S.over = k - above;
-        } else {
-          S.list[atomicAdd(&S.n_list, 1)] = tid;
-        }
+#pragma unroll
+      for (int o = LP_LANES / 2; o > 0; o >>= 1) {
+        above += __shfl_xor_sync(0xffffffffu, above, o);
+        same += __shfl_xor_sync(0xffffffffu, same, o);
+      }
+      if (lane % LP_LANES == 0 && above < k && g != 0u) {
+        if (above + same > k)  // more groups share this maximum than belong to the best k
+          S.over = k - above;  // (the same from all of them)
+        else
+          S.list[atomicAdd(&S.n_list, 1)] = grp;
         if (above + same >= k) S.kz = g;  // (the same value from all that write it)
       }
     }
@@ -240,7 +245,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
     lp_key_t K = (lp_key_t)S.kz << 32;
     if (S.over > 0) {  // (uniform) of the groups that share it, those with the lowest indices
       lp_key_t g = 0ull;
-      if (my_z == S.kz && S.gz[tid >> 3] == S.kz) {
+      if (my_z == S.kz && S.gz[tid / LP_LANES] == S.kz) {
         int i = T.at == LP_HEAD ? lo + tid : v0 + 4 * nv + tid;
         if (T.at >= 0) {
           i = INT_MAX;
@@ -255,8 +260,8 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
         g = lp_key(T.z, i);
       }
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
-      if ((lane & 7) == 0) S.group[tid >> 3] = g;
+      for (int o = LP_LANES / 2; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
+      if (lane % LP_LANES == 0) S.group[tid / LP_LANES] = g;
       __syncthreads();
       if (tid < LP_GROUPS && S.group[tid] != 0ull) {
         int above = 0;
@@ -281,14 +286,14 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
     };
     // the listed groups' vectors, dealt to all threads, LOOKS loads at a time
     constexpr int LOOKS = 4;
-    const int per_group = 8 * ((nv + LP_THREADS - 1) / LP_THREADS), looks = S.n_list * per_group;
+    const int per_group = LP_LANES * ((nv + LP_THREADS - 1) / LP_THREADS), looks = S.n_list * per_group;
     for (int e0 = tid; e0 < looks; e0 += LOOKS * LP_THREADS) {
       float4 w[LOOKS];
       int at[LOOKS];
 #pragma unroll
       for (int u = 0; u < LOOKS; ++u) {
         const int e = e0 + u * LP_THREADS, g = e / per_group, j = e - g * per_group;
-        at[u] = e < looks ? S.list[g] * 8 + (j & 7) + (j >> 3) * LP_THREADS : nv;
+        at[u] = e < looks ? S.list[g] * LP_LANES + j % LP_LANES + j / LP_LANES * LP_THREADS : nv;
         if (at[u] < nv) w[u] = __ldg(xv + at[u]);
       }
 #pragma unroll
@@ -311,6 +316,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
       for (int i = tid; i < found; i += LP_THREADS) {
         const lp_key_t key = S.cand[i];
         int above = 0;
+#pragma unroll 8
         for (int j = 0; j < found; ++j) above += S.cand[j] > key;
         if (above < k) S.top[above] = key;
       }
@@ -327,18 +333,17 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
         if (tid == 0) S.top[j] = last;
       }
     }
-    if (tid == 0) S.n_top = k;
+    if (tid >= k && tid < GSDLQ_MAX_TOP) S.top[tid] = 0ull;  // below every key
   }
 
   // ---- the row
   if (cluster > 1) {
     cluster_sync_all();  // every CTA's part and top are written
     if (rank == 0) {
-      const uint32_t at_part = smem_u32(&S.part), at_n = smem_u32(&S.n_top), at_top = smem_u32(S.top);
+      const uint32_t at_part = smem_u32(&S.part), at_top = smem_u32(S.top);
       if (tid < cluster) {
         const uint32_t p = mapa_shared(at_part, tid);
         S.parts[tid] = {ld_cluster_f32(p), ld_cluster_f32(p + 4), ld_cluster_f32(p + 8)};
-        if (J.top > 0) S.counts[tid] = __float_as_int(ld_cluster_f32(mapa_shared(at_n, tid)));
       }
       if (J.top > 0 && tid < cluster * GSDLQ_MAX_TOP) {
         const int q = tid / GSDLQ_MAX_TOP, j = tid % GSDLQ_MAX_TOP;
@@ -375,24 +380,22 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
     if (tid < J.top) put(tid, S.top[tid]);
   } else if (J.top > 0 && tid < cluster * GSDLQ_MAX_TOP) {
     // the place of entry j of CTA q's list: j, and what the other lists have above it
+    // (all searches side by side: list o has at[o] keys above it)
     const int q = tid / GSDLQ_MAX_TOP, j = tid % GSDLQ_MAX_TOP;
-    if (j < S.counts[q]) {
-      const lp_key_t key = S.all[q][j];
-      int at = j;
-      for (int o = 0; o < cluster; ++o) {
-        if (o == q) continue;
-        int a = 0, b = S.counts[o];
-        while (a < b) {
-          const int mid = (a + b) / 2;
-          if (S.all[o][mid] > key)
-            a = mid + 1;
-          else
-            b = mid;
-        }
-        at += a;
-      }
-      if (at < J.top) put(at, key);
-    }
+    const lp_key_t key = S.all[q][j];
+    int at[LP_MAX_CLUSTER];
+#pragma unroll
+    for (int o = 0; o < LP_MAX_CLUSTER; ++o) at[o] = 0;
+#pragma unroll
+    for (int step = GSDLQ_MAX_TOP / 2; step > 0; step >>= 1)
+#pragma unroll
+      for (int o = 0; o < LP_MAX_CLUSTER; ++o)
+        if (o < cluster && S.all[o][at[o] + step - 1] > key) at[o] += step;
+    int place = 0;
+#pragma unroll
+    for (int o = 0; o < LP_MAX_CLUSTER; ++o)
+      if (o < cluster) place += at[o] + (at[o] == GSDLQ_MAX_TOP - 1 && S.all[o][GSDLQ_MAX_TOP - 1] > key);
+    if (key != 0ull && place < J.top) put(place, key);
   }
 }
 
@@ -409,9 +412,10 @@ extern "C" int gsdlq_logprobs_rows(const gsdlq_logprobs_job_t* job, gsdlq_stream
   if (J.top < 0 || J.top > GSDLQ_MAX_TOP || J.top > J.n || (J.top > 0 && (!J.top_ids || !J.top_logprobs)))
     return GSDLQ_ERR_INVALID;
   if (!J.ids && !J.entropy && J.top == 0) return GSDLQ_ERR_INVALID;
-  // CTAs a row: as many as run at once, two an SM, none with less than 2048 logits
+  // CTAs a row: as many as run at once, two an SM, none with less than 8192 logits (a row of 32768 with 5
+  // alternatives: 7.6 us with 8 CTAs, 6.6 with 4, 7.1 with 2, 7.6 with 1; of 151936 with 20: 10.2 with 8, 11.8 with 4)
   int cluster = 1;
-  while (cluster < LP_MAX_CLUSTER && (long long)J.rows * cluster * 2 <= 2 * num_sms() && J.n / (cluster * 2) >= 2048)
+  while (cluster < LP_MAX_CLUSTER && (long long)J.rows * cluster * 2 <= 2 * num_sms() && J.n / (cluster * 2) >= 8192)
     cluster *= 2;
   if ((long long)J.rows * cluster > INT32_MAX) return GSDLQ_ERR_INVALID;
   return launch_pdl(logprobs_rows_kernel, (unsigned)(J.rows * cluster), LP_THREADS, 0, static_cast<cudaStream_t>(stream),
