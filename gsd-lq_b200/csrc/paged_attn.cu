@@ -30,7 +30,7 @@ namespace gsdlq {
 // so that one product gives both parts and c[0] + c[2], c[1] + c[3] are the sums.  With A = q, B = K^T the score
 // fragment is already p's A fragment for the second product, B = V.  The second product starts from zero each
 // unit and is added to fp32 registers, which keeps the tensor core's truncating accumulation short.
-constexpr int PA_MAX_CTAS = 480;  // largest grid of an attention launch
+constexpr int PA_MAX_CTAS = 320;  // largest grid of an attention launch
 constexpr int PA_PER_SM = 2;
 constexpr int PA_GROUP = 8;       // query heads of one kv head taken together
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
@@ -53,9 +53,11 @@ inline size_t attention_paged_counters(int rows, int n_heads, int n_kv) {
   const size_t items = (size_t)rows * n_kv * ((n_heads / n_kv + PA_GROUP - 1) / PA_GROUP);
   return (items * sizeof(unsigned) + 15) / 16 * 16;
 }
-// counters of the items, then two partial results per CTA (its first and its last item)
+// counters of the items, then two partial results per CTA (its first and its last item), in the form for rows that
+// share sequences one per warp
 inline size_t attention_paged_work(int rows, int n_heads, int n_kv, int hd) {
-  return attention_paged_counters(rows, n_heads, n_kv) + sizeof(float) * (size_t)PA_MAX_CTAS * 2 * PA_GROUP * (hd + 2);
+  return attention_paged_counters(rows, n_heads, n_kv) +
+         sizeof(float) * (size_t)PA_MAX_CTAS * 2 * PA_WARPS * PA_GROUP * (hd + 2);
 }
 
 template <bool BF16>
@@ -116,6 +118,175 @@ __device__ __forceinline__ uint32_t pa_at(int j, int c) {
   return (uint32_t)(j * (HD * 2) + ((c ^ x) << 4));
 }
 
+// Up to eight query columns -- heads, or heads of several rows -- in a warp; a lane's column is lane / 4.
+template <int HD, bool BF16>
+struct PaColumns {
+  static constexpr int TOK = pa_tok(HD), CH = HD / 8, KS = HD / 16;
+  static constexpr float P_SHIFT = BF16 ? 0.f : 11.f;
+  uint32_t qa[KS][4], ql[KS][2];  // q as A fragments
+  float scale, m, l;              // of the log2 scores; largest score so far, before the scale; this lane's sum of weights
+  float acc[CH][2];
+  typedef float2 Raw[KS][2];      // this lane's entries of its column's q, as loaded
+
+  static __device__ __forceinline__ void load(Raw& x, const float* q) {  // q of the column
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) x[k][i] = *reinterpret_cast<const float2*>(q + 2 * (threadIdx.x & 3) + k * 16 + i * 8);
+  }
+  __device__ __forceinline__ void begin(const Raw& x, float sm_scale) {
+    scale = sm_scale * 1.4426950408889634f;
+    float up = copysignf(1.f, scale);  // scores with the sign of the scale: the largest has the largest weight
+    if (!BF16) {
+      // the largest entry to [2^14, 2^15), by a power of two (a row below 2^-112 not quite so far)
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) top = fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y)));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = top > 0.f && top < INFINITY ? min(14 - ilogbf(top), 126) : 0;  // -113 .. 126
+      up *= __int_as_float((127 + e) << 23);
+      scale *= __int_as_float((127 - e) << 23);
+    }
+    scale = fmaxf(fabsf(scale), FLT_MIN);  // (a masked position's -inf stays -inf)
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        pa_split<BF16>(x[k][i].x * up, x[k][i].y * up, qa[k][2 * i], qa[k][2 * i + 1], ql[k][i]);
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int n = 0; n < CH; ++n) acc[n][0] = acc[n][1] = 0.f;
+  }
+  // scores of a unit, 8 positions a step; k0: this lane's row of the tile's first matrices
+  __device__ __forceinline__ void scores(float (&p)[TOK / 8][2], uint32_t k0) const {
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    float s[TOK / 8][4];
+#pragma unroll
+    for (int k = 0; k < KS; k += 2) {
+#pragma unroll
+      for (int n = 0; n < TOK / 8; ++n) {
+        uint32_t b[4];
+        pa_ldm(b, (k0 ^ (k << 5)) + n * (HD * 16));
+        if (k == 0)
+          pa_mma<BF16>(s[n], qa[k], b[0], b[1], zero);
+        else
+          pa_mma<BF16>(s[n], qa[k], b[0], b[1], s[n]);
+        pa_mma<BF16>(s[n], qa[k + 1], b[2], b[3], s[n]);
+        if constexpr (BF16) {
+          const uint32_t a0[4] = {ql[k][0], 0u, ql[k][1], 0u}, a1[4] = {ql[k + 1][0], 0u, ql[k + 1][1], 0u};
+          pa_mma<BF16>(s[n], a0, b[0], b[1], s[n]);
+          pa_mma<BF16>(s[n], a1, b[2], b[3], s[n]);
+        }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < TOK / 8; ++n) {
+      p[n][0] = s[n][0] + s[n][2];
+      p[n][1] = s[n][1] + s[n][3];
+    }
+  }
+  struct Weights {
+    uint32_t a[TOK / 16][4], lo[TOK / 16][2];  // as A fragments
+    float f;                                   // what the earlier results are worth now
+  };
+  // the weights of scores p (-inf: masked); the running maximum and sum move on
+  __device__ __forceinline__ void weights(Weights& W, const float (&p)[TOK / 8][2]) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < TOK / 8; ++n) top = fmaxf(top, fmaxf(p[n][0], p[n][1]));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn;
+    W.f = ex2_ftz((m - ref) * scale);
+    const float shift = fmaf(-ref, scale, P_SHIFT);
+    m = mn;
+    float ps = 0.f;
+#pragma unroll
+    for (int n = 0; n < TOK / 8; ++n) {
+      const float p0 = ex2_ftz(fmaf(p[n][0], scale, shift)), p1 = ex2_ftz(fmaf(p[n][1], scale, shift));
+      ps += p0 + p1;
+      pa_split<BF16>(p0, p1, W.a[n / 2][(n & 1) * 2], W.a[n / 2][(n & 1) * 2 + 1], W.lo[n / 2][n & 1]);
+    }
+    l = fmaf(l, W.f, ps);
+  }
+  // weighted values, 16 positions a step; v0: this lane's row of the tile's first matrices
+  __device__ __forceinline__ void values(const Weights& W, uint32_t v0) {
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < CH; n += 2) {
+      float o0[4], o1[4];
+#pragma unroll
+      for (int k = 0; k < TOK / 16; ++k) {
+        uint32_t b[4];
+        pa_ldm_trans(b, (v0 ^ (n << 4)) + k * (HD * 32));
+        if (k == 0) {
+          pa_mma<BF16>(o0, W.a[k], b[0], b[1], zero);
+          pa_mma<BF16>(o1, W.a[k], b[2], b[3], zero);
+        } else {
+          pa_mma<BF16>(o0, W.a[k], b[0], b[1], o0);
+          pa_mma<BF16>(o1, W.a[k], b[2], b[3], o1);
+        }
+        if constexpr (BF16) {
+          const uint32_t a[4] = {W.lo[k][0], 0u, W.lo[k][1], 0u};
+          pa_mma<BF16>(o0, a, b[0], b[1], o0);
+          pa_mma<BF16>(o1, a, b[2], b[3], o1);
+        }
+      }
+      acc[n][0] = fmaf(acc[n][0], W.f, o0[0] + o0[2]);
+      acc[n][1] = fmaf(acc[n][1], W.f, o0[1] + o0[3]);
+      acc[n + 1][0] = fmaf(acc[n + 1][0], W.f, o1[0] + o1[2]);
+      acc[n + 1][1] = fmaf(acc[n + 1][1], W.f, o1[1] + o1[3]);
+    }
+  }
+  // this lane's sums over its column's four lanes
+  __device__ __forceinline__ void finish() {
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+  }
+};
+__device__ __forceinline__ float pa_inverse(float x) { return x > 0.f ? 1.f / x : (x == 0.f ? 0.f : NAN); }  // 0: no position left
+
+// Four values (the e-th four of column c) of an item that n_parts CTAs from `first` on hold: a CTA's part lies in its
+// second place where the item begins, else in the first.  A place: [PA_GROUP][HD] weighted sums, then the columns'
+// (maximum, sum of weights); places are `slot` floats apart.
+template <int HD>
+__device__ __forceinline__ float4 pa_join(const float* part, size_t slot, int first, int n_parts, int c, int e) {
+  constexpr int BATCH = 8;  // parts whose loads are in flight together
+  float M = -INFINITY, L = 0.f;
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n_parts; i0 += BATCH) {
+    float4 o[BATCH];
+    float2 ml[BATCH];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int q = min(i0 + i, n_parts - 1);
+      const float* const at = part + ((size_t)(first + q) * 2 + (q == 0)) * slot;
+      o[i] = __ldcg(reinterpret_cast<const float4*>(at + c * HD) + e);
+      ml[i] = __ldcg(reinterpret_cast<const float2*>(at + PA_GROUP * HD) + c);
+      if (i0 + i >= n_parts) ml[i].x = -INFINITY;
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i].x);
+    const float ref = top == -INFINITY ? 0.f : top, f0 = ex2_ftz(M - ref);
+    M = top;
+    L *= f0;
+    A = make_float4(A.x * f0, A.y * f0, A.z * f0, A.w * f0);
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float f = ex2_ftz(ml[i].x - ref);
+      L = fmaf(ml[i].y, f, L);
+      A = make_float4(fmaf(o[i].x, f, A.x), fmaf(o[i].y, f, A.y), fmaf(o[i].z, f, A.z), fmaf(o[i].w, f, A.w));
+    }
+  }
+  const float inv = pa_inverse(L);
+  return make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
+}
+
 // a walk over a CTA's run, segment by segment: the part of an item that lies in it
 struct PagedWalk {
   int row, seq, len, tiles;  // tiles: units of each of the row's items
@@ -132,9 +303,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
   constexpr int TOK = pa_tok(HD);
   constexpr int TILE = TOK * HD * 2;       // bytes of a tile
   constexpr int CH = HD / 8;               // 16-byte chunks of a position
-  constexpr int KS = HD / 16;              // k steps of the first product
   constexpr int TPL = TOK / 32;            // positions a lane looks up
-  constexpr float P_SHIFT = BF16 ? 0.f : 11.f;
   typedef typename std::conditional<TOK == 64, unsigned long long, unsigned>::type mask_t;  // a bit per position
   constexpr mask_t FULL = ~(mask_t)0;
   extern __shared__ __align__(1024) uint8_t pa_smem[];
@@ -325,7 +494,9 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
   };
 
   // ---- queries of a segment, as loaded
-  float2 x[KS][2];
+  typedef PaColumns<HD, BF16> Cols;
+  Cols C;
+  typename Cols::Raw x;
   auto seg_heads = [&](const PagedWalk& w, int& head0) {  // first query head, and how many
     const int g = subs == 1 ? w.item : w.item / subs, sub = subs == 1 ? 0 : w.item - g * subs;
     head0 = g * gq_all + sub * PA_GROUP;
@@ -337,12 +508,8 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     } while (cur.step == 1 && cur.t >= cur.b);
     int head0;
     const int gq = seg_heads(cur, head0);
-    const float* q = J.q + cur.row * (J.q_stride ? (size_t)J.q_stride : (size_t)J.n_heads * HD) +
-                     (size_t)(head0 + min(lane >> 2, gq - 1)) * HD + 2 * (lane & 3);
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) x[k][i] = *reinterpret_cast<const float2*>(q + k * 16 + i * 8);
+    Cols::load(x, J.q + cur.row * (J.q_stride ? (size_t)J.q_stride : (size_t)J.n_heads * HD) +
+                      (size_t)(head0 + min(lane >> 2, gq - 1)) * HD);
     return true;
   };
 
@@ -362,68 +529,16 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
   // this lane's rows of the first K and V matrices
   const uint32_t k0 = kt + pa_at<HD>(lane & 7, lane >> 3), vt0 = kt + TILE + pa_at<HD>(lane & 15, lane >> 4);
   while (have) {
-    // q of this lane's head as A fragments
-    uint32_t qa[KS][4], ql[KS][2];
-    float s_scale = J.sm_scale * 1.4426950408889634f;
-    {
-      float up = copysignf(1.f, s_scale);  // scores with the sign of the scale: the largest has the largest weight
-      if (!BF16) {
-        // the largest entry to [2^14, 2^15), by a power of two (a row below 2^-112 not quite so far)
-        float top = 0.f;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) top = fmaxf(top, fmaxf(fabsf(x[k][i].x), fabsf(x[k][i].y)));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = top > 0.f && top < INFINITY ? min(14 - ilogbf(top), 126) : 0;  // -113 .. 126
-        up *= __int_as_float((127 + e) << 23);
-        s_scale *= __int_as_float((127 - e) << 23);
-      }
-      s_scale = fmaxf(fabsf(s_scale), FLT_MIN);  // (a masked position's -inf stays -inf)
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          pa_split<BF16>(x[k][i].x * up, x[k][i].y * up, qa[k][2 * i], qa[k][2 * i + 1], ql[k][i]);
-    }
-    float m = -INFINITY, l = 0.f, acc[CH][2];
-#pragma unroll
-    for (int n = 0; n < CH; ++n) acc[n][0] = acc[n][1] = 0.f;
-    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    C.begin(x, J.sm_scale);
     for (; cur.t < cur.b; cur.t += cur.step) {
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncwarp();
-      // scores, 8 positions a step
-      float s[TOK / 8][4];
-#pragma unroll
-      for (int k = 0; k < KS; k += 2) {
-#pragma unroll
-        for (int n = 0; n < TOK / 8; ++n) {
-          uint32_t b[4];
-          pa_ldm(b, (k0 ^ (k << 5)) + n * (HD * 16));
-          if (k == 0)
-            pa_mma<BF16>(s[n], qa[k], b[0], b[1], zero);
-          else
-            pa_mma<BF16>(s[n], qa[k], b[0], b[1], s[n]);
-          pa_mma<BF16>(s[n], qa[k + 1], b[2], b[3], s[n]);
-          if constexpr (BF16) {
-            const uint32_t a0[4] = {ql[k][0], 0u, ql[k][1], 0u}, a1[4] = {ql[k + 1][0], 0u, ql[k + 1][1], 0u};
-            pa_mma<BF16>(s[n], a0, b[0], b[1], s[n]);
-            pa_mma<BF16>(s[n], a1, b[2], b[3], s[n]);
-          }
-        }
-      }
+      float p[TOK / 8][2];
+      C.scores(p, k0);
       __syncwarp();  // the K tile is read
       valid_next = resolve(U, slot);
       head = U.head;
       copy(kp, head, slot, valid_next, 0);
-      // the scores, their maximum, the weights as powers of 2
-      float top = -INFINITY, p[TOK / 8][2];
-#pragma unroll
-      for (int n = 0; n < TOK / 8; ++n)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) p[n][j] = s[n][j] + s[n][j + 2];
       if (valid != FULL) {
         const mask_t mine = valid >> (2 * (lane & 3));
 #pragma unroll
@@ -432,69 +547,27 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
           for (int j = 0; j < 2; ++j)
             if (!((mine >> (n * 8 + j)) & 1)) p[n][j] = -INFINITY;
       }
-#pragma unroll
-      for (int n = 0; n < TOK / 8; ++n) top = fmaxf(top, fmaxf(p[n][0], p[n][1]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // m: the largest score so far, before the scale
-      const float mn = fmaxf(m, top), ref = mn == -INFINITY ? 0.f : mn, f = ex2_ftz((m - ref) * s_scale);
-      const float shift = fmaf(-ref, s_scale, P_SHIFT);
-      m = mn;
-      uint32_t pa[TOK / 16][4], pl[TOK / 16][2];
-      float ps = 0.f;
-#pragma unroll
-      for (int n = 0; n < TOK / 8; ++n) {
-        const float p0 = ex2_ftz(fmaf(p[n][0], s_scale, shift)), p1 = ex2_ftz(fmaf(p[n][1], s_scale, shift));
-        ps += p0 + p1;
-        pa_split<BF16>(p0, p1, pa[n / 2][(n & 1) * 2], pa[n / 2][(n & 1) * 2 + 1], pl[n / 2][n & 1]);
-      }
-      l = fmaf(l, f, ps);
-      // weighted values, 16 positions a step
+      typename Cols::Weights W;
+      C.weights(W, p);
       asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncwarp();
-#pragma unroll
-      for (int n = 0; n < CH; n += 2) {
-        float o0[4], o1[4];
-#pragma unroll
-        for (int k = 0; k < TOK / 16; ++k) {
-          uint32_t b[4];
-          pa_ldm_trans(b, (vt0 ^ (n << 4)) + k * (HD * 32));
-          if (k == 0) {
-            pa_mma<BF16>(o0, pa[k], b[0], b[1], zero);
-            pa_mma<BF16>(o1, pa[k], b[2], b[3], zero);
-          } else {
-            pa_mma<BF16>(o0, pa[k], b[0], b[1], o0);
-            pa_mma<BF16>(o1, pa[k], b[2], b[3], o1);
-          }
-          if constexpr (BF16) {
-            const uint32_t a[4] = {pl[k][0], 0u, pl[k][1], 0u};
-            pa_mma<BF16>(o0, a, b[0], b[1], o0);
-            pa_mma<BF16>(o1, a, b[2], b[3], o1);
-          }
-        }
-        acc[n][0] = fmaf(acc[n][0], f, o0[0] + o0[2]);
-        acc[n][1] = fmaf(acc[n][1], f, o0[1] + o0[3]);
-        acc[n + 1][0] = fmaf(acc[n + 1][0], f, o1[0] + o1[2]);
-        acc[n + 1][1] = fmaf(acc[n + 1][1], f, o1[1] + o1[3]);
-      }
+      C.values(W, vt0);
       __syncwarp();  // the V tile is read
       copy(vp, head, slot, valid_next, 1);
       valid = valid_next;
       look(U);
     }
     // ---- the segment's result
-    l += __shfl_xor_sync(0xffffffffu, l, 1);
-    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    C.finish();
     int head0;
     const int gq = seg_heads(cur, head0), h = lane >> 2;
     float* const out = J.out + ((size_t)cur.row * J.n_heads + head0) * HD;
-    auto inverse = [](float x) { return x > 0.f ? 1.f / x : (x == 0.f ? 0.f : NAN); };  // 0: no position left
     if (cur.step == 1) {  // all of the item, in this warp
       if (h < gq) {
-        const float inv = inverse(l);
+        const float inv = pa_inverse(C.l);
 #pragma unroll
         for (int n = 0; n < CH; ++n)
-          *reinterpret_cast<float2*>(out + h * HD + n * 8 + 2 * (lane & 3)) = make_float2(acc[n][0] * inv, acc[n][1] * inv);
+          *reinterpret_cast<float2*>(out + h * HD + n * 8 + 2 * (lane & 3)) = make_float2(C.acc[n][0] * inv, C.acc[n][1] * inv);
       }
       have = next_seg();
       continue;
@@ -511,10 +584,10 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
 #pragma unroll
         for (int n = 0; n < DIMS / 8; ++n)
           *reinterpret_cast<float2*>(&S.acc[warp][h][n * 8 + 2 * (lane & 3)]) =
-              make_float2(acc[d0 / 8 + n][0], acc[d0 / 8 + n][1]);
+              make_float2(C.acc[d0 / 8 + n][0], C.acc[d0 / 8 + n][1]);
         if (d0 == 0 && (lane & 3) == 0) {
-          S.m[warp][h] = m * s_scale;
-          S.l[warp][h] = l;
+          S.m[warp][h] = C.m * C.scale;
+          S.l[warp][h] = C.l;
         }
       }
       if (d0 + DIMS == HD) have = next_seg();
@@ -535,7 +608,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
           A = make_float4(fmaf(o.x, f, A.x), fmaf(o.y, f, A.y), fmaf(o.z, f, A.z), fmaf(o.w, f, A.w));
         }
         if (whole) {
-          const float inv = inverse(L);
+          const float inv = pa_inverse(L);
           *reinterpret_cast<float4*>(out + hh * HD + d0 + d) = make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
         } else {
           __stcg(reinterpret_cast<float4*>(mine + hh * HD + d0 + d), A);
@@ -551,39 +624,9 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
       __syncthreads();
       if (S.last) {
         __threadfence();
-        constexpr int BATCH = 8;  // parts whose loads are in flight together
-        for (int e = tid; e < gq * HD / 4; e += PA_THREADS) {
-          const int hh = e / (HD / 4);
-          float M = -INFINITY, L = 0.f;
-          float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int i0 = 0; i0 < n_parts; i0 += BATCH) {
-            float4 o[BATCH];
-            float2 ml[BATCH];
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-              const int q = min(i0 + i, n_parts - 1);
-              const float* const at = part + ((size_t)(first + q) * 2 + (q == 0)) * PA_GROUP * (HD + 2);
-              o[i] = __ldcg(reinterpret_cast<const float4*>(at) + e);
-              ml[i] = __ldcg(reinterpret_cast<const float2*>(at + PA_GROUP * HD) + hh);
-              if (i0 + i >= n_parts) ml[i].x = -INFINITY;
-            }
-            float top = M;
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i) top = fmaxf(top, ml[i].x);
-            const float ref = top == -INFINITY ? 0.f : top, f0 = ex2_ftz(M - ref);
-            M = top;
-            L *= f0;
-            A = make_float4(A.x * f0, A.y * f0, A.z * f0, A.w * f0);
-#pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-              const float f = ex2_ftz(ml[i].x - ref);
-              L = fmaf(ml[i].y, f, L);
-              A = make_float4(fmaf(o[i].x, f, A.x), fmaf(o[i].y, f, A.y), fmaf(o[i].z, f, A.z), fmaf(o[i].w, f, A.w));
-            }
-          }
-          const float inv = inverse(L);
-          *(reinterpret_cast<float4*>(out) + e) = make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
-        }
+        for (int e = tid; e < gq * HD / 4; e += PA_THREADS)
+          *(reinterpret_cast<float4*>(out) + e) =
+              pa_join<HD>(part, PA_GROUP * (HD + 2), first, n_parts, e / (HD / 4), e % (HD / 4));
         if (tid == 0) *count = 0u;
       }
     }
@@ -593,22 +636,345 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
 }
 
 // ---------------------------------------------------------------------------------------
+// Rows that share sequences (chunks of prompts, several drafted tokens): an item is a pack of neighbouring rows of
+// one sequence and a kv head.  The CTA's warps share the tiles of K and V, and each has rows of its own: as many as
+// fill its eight columns.  So a tile is fetched once for up to 32 rows, where the kernel above fetches it for every
+// row.  A pack is a run of rows with the same sequence inside PA_WARPS * rows_warp rows from a multiple of that
+// on, so that every CTA finds the same packs from a row's neighbours alone.  The units are the tiles up to the
+// longest row's end, dealt to the CTAs as above; a warp passes over those that lie behind all its rows.
+constexpr int PC_STAGES = 4;  // tiles of K and V on their way or in use
+constexpr int PC_OVER = 2;    // units that an item counts besides its own
+
+template <int HD>
+struct PagedChunkSmem {
+  uint8_t tile[PC_STAGES][2][pa_tok(HD) * HD * 2];  // K, V
+  unsigned valid[PC_STAGES][PA_WARPS];              // of the positions that a warp has looked up
+  int seq[PA_THREADS], len[PA_THREADS];             // of the rows, while the packs are counted
+  int warp_sum[PA_WARPS];
+  int row, base, last;
+};
+
+struct PagedPack {
+  int row, n, seq, len, tiles;  // its rows, their sequence, the longest one's positions and units
+  int own;                      // positions of this lane's row
+  int item, s, a, b, t;         // as in PagedWalk; t: the next unit
+};
+
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
+    attention_paged_chunk_kernel(const __grid_constant__ gsdlq_paged_attn_job_t J, int subs, int page_shift, int rows_warp) {
+  constexpr int TOK = pa_tok(HD), CH = HD / 8;
+  constexpr int TILE = TOK * HD * 2;
+  constexpr int TOKW = TOK / PA_WARPS;  // positions of a tile that a warp looks up and copies
+  typedef typename std::conditional<TOK == 64, unsigned long long, unsigned>::type mask_t;
+  constexpr mask_t FULL = ~(mask_t)0;
+  extern __shared__ __align__(1024) uint8_t pa_smem[];
+  PagedChunkSmem<HD>& S = *reinterpret_cast<PagedChunkSmem<HD>*>(pa_smem);
+  const gsdlq_paged_kv_t& kv = J.kv;
+  const int tid = threadIdx.x, lane = tid & 31, cta = blockIdx.x;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  const int gq_all = J.n_heads / kv.n_kv_heads, items_row = kv.n_kv_heads * subs;
+  const int group = PA_WARPS * rows_warp;  // rows of a pack; divides 32
+  const size_t kw = (size_t)kv.n_kv_heads * HD;
+  // this lane's column: row rl of its warp's, query head hl of the item's
+  const int gq_max = min(gq_all, PA_GROUP), rl = (lane >> 2) / gq_max, hl = (lane >> 2) - rl * gq_max;
+
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // ---- the launch's units, this CTA's run of them, and the pack where it begins
+  auto pack_units = [&](int r0, bool flag) {  // of the pack that row r0 + tid leads, else 0
+    const int r = r0 + tid;
+    __syncthreads();
+    if (r < J.rows) {
+      const PagedRow pr = paged_row(kv, J.row_seq, J.pos, r, flag);
+      S.seq[tid] = pr.seq;
+      S.len[tid] = pr.len;
+    }
+    __syncthreads();
+    if (r >= J.rows || (tid % group != 0 && S.seq[tid - 1] == S.seq[tid])) return 0;
+    int len = S.len[tid];
+    for (int i = tid + 1; i % group != 0 && r0 + i < J.rows && S.seq[i] == S.seq[tid]; ++i) len = max(len, S.len[i]);
+    return len > 0 ? ((len + TOK - 1) / TOK + PC_OVER) * items_row : 0;
+  };
+  auto scan = [&](int n, int& total) {  // exclusive, over the CTA
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += x;
+    }
+    if (lane == 31) S.warp_sum[warp] = inc;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < PA_WARPS; ++w) {
+      before += w < warp ? S.warp_sum[w] : 0;
+      total += S.warp_sum[w];
+    }
+    return before + inc - n;
+  };
+  int units = 0, n0 = 0, base0 = 0;
+  for (int r0 = 0; r0 < J.rows; r0 += PA_THREADS) {
+    const int n = pack_units(r0, cta == 0);
+    int total;
+    const int b = scan(n, total);
+    if (r0 == 0) {
+      n0 = n;
+      base0 = b;
+    }
+    units += total;
+  }
+  const int per = max((units + (int)gridDim.x - 1) / (int)gridDim.x, PC_OVER + 1);
+  const long long v0l = (long long)per * cta;
+  const int v0 = v0l < units ? (int)v0l : units, v1 = min(v0 + per, units);
+  for (int r = cta; r < J.rows; r += gridDim.x)  // idle rows
+    if (paged_row(kv, J.row_seq, J.pos, r, false).len == 0)
+      for (int i = tid; i < J.n_heads * HD; i += PA_THREADS) J.out[(size_t)r * J.n_heads * HD + i] = 0.f;
+  if (v0 >= v1) return;
+  int before = 0;
+  for (int r0 = 0; before <= v0; r0 += PA_THREADS) {  // (ends: v0 < units)
+    int n = n0, b = base0, total = 0;
+    if (J.rows > PA_THREADS) {
+      n = pack_units(r0, false);
+      b = scan(n, total);
+    } else {
+      total = units;
+    }
+    if (before + b <= v0 && v0 < before + b + n) {
+      S.row = r0 + tid;
+      S.base = before + b;
+    }
+    before += total;
+  }
+  __syncthreads();
+
+  auto enter = [&](PagedPack& w, int row) {  // the pack that begins with `row`
+    const int r = row + lane;
+    PagedRow pr = {-1, 0};
+    const bool in = lane < group - row % group && r < J.rows;
+    if (in) pr = paged_row(kv, J.row_seq, J.pos, r, false);
+    const int seq = __shfl_sync(0xffffffffu, pr.seq, 0);
+    const unsigned same = __ballot_sync(0xffffffffu, in && pr.seq == seq);
+    w.row = row;
+    w.n = same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+    w.seq = seq;
+    w.len = __reduce_max_sync(0xffffffffu, lane < w.n ? pr.len : 0);
+    w.tiles = (w.len + TOK - 1) / TOK;
+    const int mine = warp * rows_warp + rl, own = __shfl_sync(0xffffffffu, pr.len, mine & 31);
+    w.own = rl < rows_warp && mine < w.n ? own : 0;
+  };
+  auto advance = [&](PagedPack& w) {  // to the next segment; false: the run is at its end
+    do {
+      const int end = w.s + w.tiles;
+      if (++w.item >= items_row) {
+        do {
+          if (w.row + w.n >= J.rows) return false;
+          enter(w, w.row + w.n);
+        } while (w.tiles == 0);
+        w.item = 0;
+      }
+      w.s = end + PC_OVER;
+      if (w.s >= v1) return false;
+      w.a = max(v0 - w.s, 0);
+      w.b = min(v1 - w.s, w.tiles);
+    } while (w.a >= w.b);
+    w.t = w.a;
+    return true;
+  };
+  PagedPack ahead;
+  enter(ahead, S.row);
+  ahead.item = (v0 - S.base) / (ahead.tiles + PC_OVER) - 1;
+  ahead.s = S.base + (ahead.item + 1) * (ahead.tiles + PC_OVER) - ahead.tiles;
+  ahead.t = ahead.b = 0;
+  PagedPack cur = ahead;
+  bool more = true;
+
+  // ---- the tiles
+  const uint16_t* const kp = static_cast<const uint16_t*>(kv.k) + (size_t)J.layer * kv.n_pages * kv.page_size * kw;
+  const uint16_t* const vp = static_cast<const uint16_t*>(kv.v) + (size_t)J.layer * kv.n_pages * kv.page_size * kw;
+  const uint32_t row_bytes = (uint32_t)kw * 2, tiles = smem_u32(S.tile[0][0]);
+  struct Unit {
+    int page, at, head;  // as above, of position warp * TOKW + lane
+  };
+  auto look = [&](Unit& U) {
+    U.head = U.page = -1;
+    while (more && ahead.t >= ahead.b) more = advance(ahead);
+    if (!more) return;
+    U.head = subs == 1 ? ahead.item : ahead.item / subs;
+    const int t = ahead.t * TOK + warp * TOKW + lane;
+    if (lane < TOKW && t < ahead.len) {
+      const int b = page_shift >= 0 ? t >> page_shift : t / kv.page_size;
+      U.at = t - b * kv.page_size;
+      U.page = kv.table[(size_t)ahead.seq * kv.max_blocks + b];
+      if (U.page < 0) U.page = kv.n_pages;  // missing: reported below
+    }
+    ++ahead.t;
+  };
+  const uint32_t dst0 = tiles + pa_at<HD>(warp * TOKW + lane / CH, lane % CH);
+  auto copy = [&](const Unit& U, int stage) {
+    const bool ok = paged_valid(kv, U.page);
+    if (!ok && U.page != -1) raise_flag(GSDLQ_FLAG_BAD_PAGE);
+    const unsigned valid = __ballot_sync(0xffffffffu, ok);
+    if (U.head >= 0) {
+      if (lane == 0) S.valid[stage][warp] = valid;
+      const int slot = ok ? U.page * kv.page_size + U.at : -1;
+      const size_t off = ((size_t)U.head * HD + (lane % CH) * 8) * 2;
+      const char* const ks = reinterpret_cast<const char*>(kp) + off;
+      const char* const vs = reinterpret_cast<const char*>(vp) + off;
+      const uint32_t dst = dst0 + stage * 2 * TILE;
+#pragma unroll
+      for (int it = 0; it < TOKW * CH / 32; ++it) {
+        const int j = it * (32 / CH);
+        const uint32_t x = CH >= 8 ? (uint32_t)((j & 7) << 4) : (uint32_t)(((j >> 1) & 3) << 4);
+        const int p = __shfl_sync(0xffffffffu, slot, j + lane / CH);
+        const uint32_t d = (dst ^ x) + j * (HD * 2);
+        const size_t from = (size_t)(uint32_t)max(p, 0) * row_bytes;
+        pa_cp16(d, ks + from, p < 0 ? 0 : 16);
+        pa_cp16(d + TILE, vs + from, p < 0 ? 0 : 16);
+      }
+    }
+    cp_async_commit();
+  };
+
+  // ---- queries of a segment
+  typedef PaColumns<HD, BF16> Cols;
+  Cols C;
+  typename Cols::Raw x;
+  auto first_head = [&](const PagedPack& w, int& gq) {  // of the item's query heads, and how many
+    const int g = subs == 1 ? w.item : w.item / subs, sub = subs == 1 ? 0 : w.item - g * subs;
+    gq = min(PA_GROUP, gq_all - sub * PA_GROUP);
+    return g * gq_all + sub * PA_GROUP;
+  };
+  auto next_seg = [&]() {
+    if (!advance(cur)) return false;
+    int gq;
+    const int head0 = first_head(cur, gq);
+    // (columns without a row or a head of their own repeat another's)
+    const int r = cur.row + min(warp * rows_warp + min(rl, rows_warp - 1), cur.n - 1);
+    Cols::load(x, J.q + r * (J.q_stride ? (size_t)J.q_stride : (size_t)J.n_heads * HD) + (size_t)(head0 + min(hl, gq - 1)) * HD);
+    return true;
+  };
+
+  Unit U;
+  {
+    Unit first[PC_STAGES - 1];
+#pragma unroll
+    for (int i = 0; i < PC_STAGES - 1; ++i) look(first[i]);
+#pragma unroll
+    for (int i = 0; i < PC_STAGES - 1; ++i) copy(first[i], i);
+  }
+  look(U);
+  bool have = next_seg();
+  int stage = 0;
+  constexpr size_t PLACE = (size_t)PA_WARPS * PA_GROUP * (HD + 2);  // floats of a CTA's part
+  float* const part = reinterpret_cast<float*>(static_cast<uint8_t*>(J.work) +
+                                               ((size_t)J.rows * items_row * sizeof(unsigned) + 15) / 16 * 16) +
+                      warp * PA_GROUP * (HD + 2);
+  while (have) {
+    C.begin(x, J.sm_scale);
+    for (; cur.t < cur.b; ++cur.t) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(PC_STAGES - 2) : "memory");
+      __syncthreads();  // the tile is there, and the one before it is read
+      copy(U, stage == 0 ? PC_STAGES - 1 : stage - 1);
+      look(U);
+      const int limit = cur.own - cur.t * TOK;  // positions of the tile that this lane's row has
+      if (__any_sync(0xffffffffu, limit > 0)) {
+        const uint32_t k0 = tiles + stage * 2 * TILE + pa_at<HD>(lane & 7, lane >> 3);
+        const uint32_t v0s = tiles + stage * 2 * TILE + TILE + pa_at<HD>(lane & 15, lane >> 4);
+        float p[TOK / 8][2];
+        C.scores(p, k0);
+        mask_t valid = 0;
+#pragma unroll
+        for (int w = 0; w < PA_WARPS; ++w) valid |= (mask_t)S.valid[stage][w] << (w * TOKW);
+        if (limit < TOK) valid &= limit > 0 ? ((mask_t)1 << limit) - 1 : 0;
+        if (valid != FULL) {
+          const mask_t mine = valid >> (2 * (lane & 3));
+#pragma unroll
+          for (int n = 0; n < TOK / 8; ++n)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (!((mine >> (n * 8 + j)) & 1)) p[n][j] = -INFINITY;
+        }
+        typename Cols::Weights W;
+        C.weights(W, p);
+        C.values(W, v0s);
+      }
+      stage = stage + 1 == PC_STAGES ? 0 : stage + 1;
+    }
+    // ---- the segment's result, each warp its rows'
+    C.finish();
+    int gq;
+    const int head0 = first_head(cur, gq), h = lane >> 2;
+    const bool mine = rl < rows_warp && hl < gq && warp * rows_warp + rl < cur.n;
+    if (cur.a == 0 && cur.b == cur.tiles) {
+      if (mine) {
+        const float inv = pa_inverse(C.l);
+        float* const out = J.out + ((size_t)(cur.row + warp * rows_warp + rl) * J.n_heads + head0 + hl) * HD;
+#pragma unroll
+        for (int n = 0; n < CH; ++n)
+          *reinterpret_cast<float2*>(out + n * 8 + 2 * (lane & 3)) = make_float2(C.acc[n][0] * inv, C.acc[n][1] * inv);
+      }
+      have = next_seg();
+      continue;
+    }
+    const int first = cur.s / per, n_parts = (cur.s + cur.tiles - 1) / per - first + 1;  // CTAs that hold the item
+    float* const place = part + ((size_t)cta * 2 + (cur.s >= v0)) * PLACE;
+    if (mine) {
+#pragma unroll
+      for (int n = 0; n < CH; ++n)
+        __stcg(reinterpret_cast<float2*>(place + h * HD + n * 8 + 2 * (lane & 3)), make_float2(C.acc[n][0], C.acc[n][1]));
+      if ((lane & 3) == 0) __stcg(reinterpret_cast<float2*>(place + PA_GROUP * HD) + h, make_float2(C.m * C.scale, C.l));
+    }
+    unsigned* const count = static_cast<unsigned*>(J.work) + (size_t)cur.row * items_row + cur.item;
+    const int row = cur.row, n = cur.n;
+    have = next_seg();
+    __threadfence();
+    __syncthreads();
+    if (tid == 0) S.last = atomicAdd(count, 1u) == (unsigned)n_parts - 1u;
+    __syncthreads();
+    if (S.last) {
+      __threadfence();
+      for (int e = lane; e < PA_GROUP * HD / 4; e += 32) {
+        const int c = e / (HD / 4), cr = c / gq_max, ch = c - cr * gq_max, r = warp * rows_warp + cr;
+        if (cr < rows_warp && ch < gq && r < n)
+          *(reinterpret_cast<float4*>(J.out + ((size_t)(row + r) * J.n_heads + head0 + ch) * HD) + e % (HD / 4)) =
+              pa_join<HD>(part, PLACE, first, n_parts, c, e % (HD / 4));
+      }
+      if (tid == 0) *count = 0u;
+    }
+  }
+  cp_async_wait_all();
+}
+
+// ---------------------------------------------------------------------------------------
 // host side
 template <int HD, bool BF16>
 static int launch_attention_paged(const gsdlq_paged_attn_job_t& J, int subs, cudaStream_t st) {
-  constexpr int smem = (int)sizeof(PagedAttnSmem<HD>);
-  static_assert(PA_PER_SM * (smem + 1024) <= 228 * 1024, "shared memory of the CTAs of an SM");
+  constexpr int smem = (int)sizeof(PagedAttnSmem<HD>), smem_chunk = (int)sizeof(PagedChunkSmem<HD>);
+  static_assert(PA_PER_SM * (smem + 1024) <= 228 * 1024 && PA_PER_SM * (smem_chunk + 1024) <= 228 * 1024,
+                "shared memory of the CTAs of an SM");
   static std::atomic<bool> set[64];  // the opt-in shared memory size, once per device
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return record_cuda_error(e);
   if (dev >= 64 || !set[dev].load(std::memory_order_acquire)) {
     e = cudaFuncSetAttribute(attention_paged_kernel<HD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(attention_paged_chunk_kernel<HD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               smem_chunk);
     if (e != cudaSuccess) return record_cuda_error(e);
     if (dev < 64) set[dev].store(true, std::memory_order_release);
   }
   const int grid = std::min(PA_PER_SM * num_sms(), PA_MAX_CTAS);
   const int ps = J.kv.page_size, shift = ps & (ps - 1) ? -1 : __builtin_ctz((unsigned)ps);
+  // rows share sequences on average: the tiles are worth sharing too
+  if (J.row_seq != nullptr && J.rows >= 2 * J.kv.n_seqs) {
+    const int gq = J.n_heads / J.kv.n_kv_heads;
+    const int rows_warp = gq == 1 ? 8 : gq == 2 ? 4 : gq <= 4 ? 2 : 1;  // rows whose heads fill a warp's columns
+    return launch_pdl(attention_paged_chunk_kernel<HD, BF16>, grid, PA_THREADS, smem_chunk, st, 1, J, subs, shift, rows_warp);
+  }
   return launch_pdl(attention_paged_kernel<HD, BF16>, grid, PA_THREADS, smem, st, 1, J, subs, shift);
 }
 

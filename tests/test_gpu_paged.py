@@ -111,6 +111,30 @@ def test_attention_chunk_rows_and_repeated_sequences(cuda_lib, rng):
     assert np.array_equal(got[11], got[14])
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("hd,nkv,group,page", [(128, 2, 6, 16), (64, 4, 1, 24), (32, 2, 2, 1), (64, 2, 3, 16),
+                                               (128, 1, 4, 64), (64, 1, 8, 7), (32, 1, 20, 16)])
+def test_attention_many_rows_of_few_sequences(cuda_lib, rng, kind, hd, nkv, group, page):
+    """Packs of rows: whole chunks of sequences, idle rows and changes of sequence inside them, positions in any
+    order, more rows than a block counts at once."""
+    kv = make_pool(rng, [211, 70, 1], page, nkv, hd, DTYPES[kind], layers=2)
+    rows = [(0, p) for p in range(150, 211)] + [(1, 69 - p) for p in range(33)] + [(2, 0)] * 3 + [(1, -1)] * 2
+    rows += [(int(rng.integers(0, 3)), int(rng.integers(-1, 1))) for _ in range(20)]
+    rows += [(0, int(p)) for p in rng.integers(-1, 211, 50)]
+    q = torch.from_numpy(rng.standard_normal((len(rows), nkv * group, hd)) * 2).float().cuda()
+    check_attention(kv, 1, q, [p for _, p in rows], [s for s, _ in rows])
+
+
+def test_attention_chunks_over_long_caches(cuda_lib, rng):
+    """Chunks split over many blocks and joined; the last rows of a chunk see what the first ones do not."""
+    for hd, nkv, group, n in ((128, 2, 6, 3001), (64, 3, 1, 5000), (32, 1, 4, 4100)):
+        kv = make_pool(rng, [n], 16, nkv, hd, torch.float16)
+        for rows in (2, 5, 37, 128):
+            pos = list(range(n - rows, n))
+            q = torch.from_numpy(rng.standard_normal((rows, nkv * group, hd)) * 2).float().cuda()
+            check_attention(kv, 0, q, pos, [0] * rows)
+
+
 def test_attention_strided_q_and_extreme_scores(cuda_lib, rng):
     kv = make_pool(rng, [50, 200, 7], 16, 2, 64, torch.float16)
     wide = torch.from_numpy(rng.standard_normal((3, 4 * 64 + 20))).float().cuda()
@@ -145,6 +169,17 @@ def test_attention_leaves_out_missing_pages(cuda_lib, rng):
     assert flags() == ["bad_pos"]
     assert not run_attention(kv, 0, q, [3, 3, 3], [-1, 3, 2**31 - 1]).any()
     assert flags() == ["bad_page"]
+    # the same in the form for rows that share sequences (here six and more of three)
+    q = q.repeat(3, 1, 1)
+    got = run_attention(kv, 0, q, [63, 63, 15, 62, 1, -2, kv.max_blocks * 16, 2, 2], [0, 1, 2, 0, 0, 0, 0, 3, -1])
+    k, v = rows_of(kv, 0, 2, 16)
+    want, tol = O.attention(q[2].cpu().numpy(), k, v, 0.125)
+    assert (np.abs(got[2] - want) <= tol).all() and not got[1].any() and not got[5:].any()
+    k, v = (t[0, kv.table[0, [0, 2, 3]].long()].flatten(0, 1).double().cpu().numpy() for t in (kv.k, kv.v))
+    for r, n in ((0, 48), (3, 47), (4, 2)):
+        want, tol = O.attention(q[r].cpu().numpy(), k[:n], v[:n], 0.125)
+        assert (np.abs(got[r] - want) <= tol).all()
+    assert set(flags()) == {"bad_page", "bad_pos"}
 
 
 def test_attention_offsets_past_32_bits(cuda_lib, rng):
@@ -299,7 +334,7 @@ def test_pages_random_sequences_of_operations(cuda_lib, rng):
     assert ran_out > 3 and flags() == []
 
 
-@pytest.mark.parametrize("n_pages", [1, 31, 4095, 4096, 4097, 20000])
+@pytest.mark.parametrize("n_pages", [1, 31, 4095, 4096, 4097, 20000, 270001])
 def test_pages_large_pools_and_many_rows(cuda_lib, rng, n_pages):
     """Pools over several scan steps; free pages far apart; a thousand rows."""
     from gsdlq_b200 import paged
