@@ -172,7 +172,8 @@ class PagedBatchDecoder(BatchDecoder):
         rows = max(B, m.PREFILL_CHUNK)
         self.awork = ops.attention_paged_work(self.kv, rows, m.n_heads_local)
         i32 = dict(dtype=torch.int32, device=m.device)
-        self.row_pos, self.row_seq = torch.full((m.PREFILL_CHUNK,), -1, **i32), torch.zeros(m.PREFILL_CHUNK, **i32)
+        self.row_pos = torch.full((m.PREFILL_CHUNK,), -1, **i32)
+        self.row_seq, self.row_zero = (torch.zeros(m.PREFILL_CHUNK, **i32) for _ in range(2))
         self.idle = torch.ones(B, dtype=torch.bool, device=m.device)
         self.pos.fill_(-1)
         self._logit_graph = None
@@ -244,6 +245,7 @@ class PagedBatchDecoder(BatchDecoder):
             raise ValueError("prefill past max_seq")
         m, chunk = self.m, self.m.PREFILL_CHUNK
         self.row_seq.fill_(b)
+        table = self.kv.table[b].data_ptr()
         for c in range(0, len(ids), chunk):
             part = ids[c:c + chunk]
             n, p0 = len(part), start_pos + c
@@ -254,8 +256,9 @@ class PagedBatchDecoder(BatchDecoder):
                 append, attn = self._layer_jobs(
                     "prefill", l, self._heads(buf["q"], m.n_heads_local), self._heads(buf["k"], m.n_kv_local),
                     self._heads(buf["v"], m.n_kv_local), self._heads(buf["att"], m.n_heads_local), self.row_pos,
-                    self.row_seq)
-                append.rows = attn.rows = n
+                    self.row_zero)
+                for j in (append, attn):  # the sequence alone, as sequence 0: its rows share their tiles
+                    j.rows, j.kv.table, j.kv.n_seqs = n, table, 1
                 ops.rope_kv_paged(append)
                 ops.attention_paged(attn)
 
