@@ -131,7 +131,8 @@ class PagedKV:
 
     def resized(self, n_pages: int) -> "PagedKV":
         """This cache in a pool of ``n_pages`` pages, larger or (after compact) smaller: a new pool with the pages'
-        contents, and the same table tensor and counts.  Waits for the device."""
+        contents and counts, and the same table tensor, so that this one must not be used any more.  Waits for the
+        device."""
         keep = min(int(n_pages), self.n_pages)
         if n_pages < 1:
             raise ValueError("at least one page")
@@ -183,7 +184,8 @@ class PagedBatchDecoder(BatchDecoder):
         j = self._jobs.get((key, l))
         if j is None:
             m = self.m
-            j = (ops.paged_append_job(self.kv, l, q, k, v, q, pos, m.rope_cs, row_seq),
+            # (positions at max_seq and above have no angle: reported as bad positions)
+            j = (ops.paged_append_job(self.kv, l, q, k, v, q, pos, m.rope_cs[:self.S], row_seq),
                  ops.paged_attn_job(self.kv, l, q, out, pos, 1.0 / math.sqrt(m.head_dim), self.awork, row_seq))
             self._jobs[(key, l)] = j
         return j
@@ -237,7 +239,8 @@ class PagedBatchDecoder(BatchDecoder):
 
     # ------------------------------------------------------------------ sequences
     def prefill(self, b: int, ids, start_pos: int = 0):
-        """Fill sequence b's pages with ``ids`` at positions start_pos.. (chunked tensor-core prefill)."""
+        """Fill sequence b's pages with ``ids`` at positions start_pos.. (chunked tensor-core prefill).  MemoryError
+        when the pool runs out (what came before that chunk is stored)."""
         ids = [int(t) for t in ids]
         if not 0 <= b < self.B:
             raise ValueError(f"sequence outside [0, {self.B})")
@@ -251,6 +254,8 @@ class PagedBatchDecoder(BatchDecoder):
             n, p0 = len(part), start_pos + c
             self.row_pos[:n].copy_(torch.arange(p0, p0 + n, dtype=torch.int32))
             self.kv.reserve(self.row_pos[:n], self.row_seq[:n])
+            if int(self.kv.counts[1]):
+                raise MemoryError("the page pool is exhausted")
 
             def attend(l, buf):
                 append, attn = self._layer_jobs(

@@ -125,6 +125,19 @@ def test_attention_many_rows_of_few_sequences(cuda_lib, rng, kind, hd, nkv, grou
     check_attention(kv, 1, q, [p for _, p in rows], [s for s, _ in rows])
 
 
+def test_attention_hundreds_of_sequences(cuda_lib, rng):
+    """More rows than a block counts at once, each of a sequence of its own, in order and permuted."""
+    n = 300
+    lens = [int(x) for x in rng.integers(0, 90, n)]
+    lens[7], lens[200] = 700, 1300
+    kv = make_pool(rng, lens, 16, 2, 64, torch.float16)
+    q = torch.from_numpy(rng.standard_normal((n, 6, 64)) * 2).float().cuda()
+    check_attention(kv, 0, q, [x - 1 for x in lens])
+    seq = [int(s) for s in rng.permutation(n)]
+    check_attention(kv, 0, q, [lens[s] - 1 for s in seq], seq)
+    check_attention(kv, 0, q[:40], [lens[s] - 1 for s in seq[:40]], seq[:40])
+
+
 def test_attention_chunks_over_long_caches(cuda_lib, rng):
     """Chunks split over many blocks and joined; the last rows of a chunk see what the first ones do not."""
     for hd, nkv, group, n in ((128, 2, 6, 3001), (64, 3, 1, 5000), (32, 1, 4, 4100)):

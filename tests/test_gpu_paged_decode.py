@@ -95,6 +95,11 @@ def test_generate_idle_sequences_and_page_exhaustion(cuda_lib):
     assert L.device_flags() == 0
     # no host check on single steps: a step that finds no page reports it and leaves other sequences' rows alone
     pd.free(range(4))
+    with pytest.raises(MemoryError):
+        for b in range(3):
+            pd.prefill(b, rng.integers(0, cfg["vocab_size"], 190).tolist())
+    assert L.flag_names(L.device_flags()) == ["no_page"]
+    pd.free(range(4))
     for b in range(2):
         pd.prefill(b, rng.integers(0, cfg["vocab_size"], 190).tolist())
     before = pd.kv.k.clone()

@@ -69,6 +69,9 @@ def test_attention_refusals():
                 dict(q_stride=-4), dict(out=None), dict(out=ODD4), dict(pos=None), dict(rows=0), dict(rows=5),
                 dict(n_heads=7), dict(n_heads=0), dict(work=None), dict(work=ODD4), dict(work_bytes=ok - 1)):
         assert call(**bad) == -1, bad
+    # places or units past 31 bits: refused as unsupported, before any CUDA call
+    assert call(dict(n_pages=1 << 27, page_size=16)) == -3
+    assert call(dict(page_size=1 << 10, max_blocks=1 << 24), work_bytes=ok) == -3
 
 
 def test_page_refusals():
