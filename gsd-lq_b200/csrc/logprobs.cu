@@ -15,10 +15,11 @@
 
 namespace gsdlq {
 
-// A row is read once, by a cluster of 1 to 8 CTAs that each take a contiguous part of it.  A thread keeps the
+// A row is read once, by a cluster of 1 to 8 CTAs that each take a contiguous part of it.  A warp keeps the
 // maximum m of its logits, and of the others the sums s of e^u and t of u e^u with u = (x - m) / temperature (in
-// units of ln 2): a logit above m costs a rescaling and pushes the old maximum into the sums, every other one an
-// ex2 and two additions.  Logits come in batches, so that lanes with a new maximum diverge once per batch.  Partial results (m1 >= m2) join as
+// units of ln 2): a logit costs an ex2 and two additions, a batch with a new maximum a rescaling besides, which puts
+// the old maximum into the sums.  (With a maximum per thread nearly every batch had a new one in some lane.)
+// Partial results (m1 >= m2) join as
 //   d = (m2 - m1) / temperature,  f = e^d,  s = s1 + f (s2 + 1),  t = t1 + f (t2 + d (s2 + 1)).
 //
 // Alternatives without a second pass over the row: the maxima of the 128 groups of four threads are ranked.  Every
@@ -26,7 +27,7 @@ namespace gsdlq {
 // one of the k groups whose maximum is at least K.  Only those groups' tokens are looked at again (they are in the
 // L2 cache); those at or above K -- mostly a few more than k -- are collected and ranked by counting.  Keys are
 // (z, lowest index first) with z as the sampler rounds it, so equal z (different logits can share one) go by index;
-// the groups' indices are looked up only where the k-th maximum is shared by more groups than are wanted, as in
+// the tokens' indices are looked up only where the k-th maximum is shared by more groups than are wanted, as in
 // rows with fewer unmasked tokens than k.
 constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_LANES = 4, LP_GROUPS = LP_THREADS / LP_LANES;  // groups of neighbouring lanes; >= GSDLQ_MAX_TOP
@@ -77,19 +78,15 @@ __device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b, float c) {
   return {hi.m, fmaf(f, lo.s + 1.f, hi.s), fmaf(f, fmaf(d, lo.s + 1.f, lo.t), hi.t)};
 }
 
-struct LpThread {
-  LpSums a;
-  float near;    // a batch whose maximum reaches it may hold a better z
-  float z;       // the best z (-inf: nothing yet) ...
-  int at, vecs;  // ... and the batch that holds its first index: `vecs` vectors from `at` on
+// What a warp has read of its part: the lanes share the maximum m as reference; `holds` says in which lane it lies.
+struct LpWarp {
+  float m, s, t;  // s and t: this lane's, without the maximum
+  bool holds;
+  float top;      // this lane's largest logit (-inf: nothing yet)
 };
-constexpr int LP_HEAD = -1, LP_TAIL = -2;  // `at` of the single logits before and behind the vectors
-
-// N logits in the order of their indices.  A new maximum changes places with the old one, so that what is added
-// to the sums is again everything but the maximum.  (Lanes that find one wait for nobody more than once per batch;
-// logit by logit nearly every one is a new maximum in some lane.)
+// clean N logits; -inf for those that are not there
 template <int N>
-__device__ __forceinline__ void lp_add(LpThread& T, float (&x)[N], int at, int vecs, float temp, float c) {
+__device__ __forceinline__ void lp_clean(float (&x)[N]) {
   float wild = 0.f;  // not finite if a logit is not
 #pragma unroll
   for (int k = 0; k < N; ++k) wild = fmaf(x[k], 0.f, wild);
@@ -97,37 +94,41 @@ __device__ __forceinline__ void lp_add(LpThread& T, float (&x)[N], int at, int v
 #pragma unroll
     for (int k = 0; k < N; ++k) x[k] = lp_clean(x[k]);
   }
+}
+// N logits of each lane (-inf: none).  Only a new maximum of the whole warp costs more than the sums.
+template <int N>
+__device__ __forceinline__ void lp_add(LpWarp& T, float (&x)[N], float c) {
   float top = x[0];
 #pragma unroll
   for (int k = 1; k < N; ++k) top = fmaxf(top, x[k]);
-  if (top >= T.near) {
-    const float z = lp_z(top, temp);
-    if (z > T.z) {
-      T.z = z;
-      T.at = at;
-      T.vecs = vecs;
-    }
-    if (top > T.a.m) {
-      const float f = ex2_ftz(fmaxf((T.a.m - top) * c, -200.f)), d = fmaxf((T.a.m - top) * c, -200.f);
-      T.a.t = f * fmaf(d, T.a.s, T.a.t);
-      T.a.s *= f;
-      bool placed = false;
+  T.top = fmaxf(T.top, top);
+  const float wtop = key_to_float(__reduce_max_sync(0xffffffffu, ordered_key(top + 0.0f)));
+  if (wtop > T.m) {
+    const float d = fmaxf((T.m - wtop) * c, -200.f), f = ex2_ftz(d), s1 = T.s + (T.holds ? 1.f : 0.f);
+    T.t = f * fmaf(d, s1, T.t);
+    T.s = f * s1;
+    T.m = wtop;
+    T.holds = __ffs(__ballot_sync(0xffffffffu, top == wtop)) - 1 == (int)(threadIdx.x & 31);
+    if (T.holds) {
+      bool out = false;  // the first one that equals it is the maximum, which the sums leave out
 #pragma unroll
       for (int k = 0; k < N; ++k) {
-        const bool it = !placed && x[k] == top;
-        placed |= it;
-        x[k] = it ? T.a.m : x[k];  // -inf at first, which adds nothing
+        const bool it = !out && x[k] == wtop;
+        out |= it;
+        x[k] = it ? -INFINITY : x[k];
       }
-      T.a.m = top;
-      T.near = lp_below(top);
     }
   }
+  // (four of each sum, so that a chain of additions is short)
+  float s4[4] = {0.f, 0.f, 0.f, 0.f}, t4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int k = 0; k < N; ++k) {
-    const float d = fmaxf((x[k] - T.a.m) * c, -200.f), e = ex2_ftz(d);
-    T.a.s += e;
-    T.a.t = fmaf(e, d, T.a.t);
+    const float d = fmaxf((x[k] - T.m) * c, -200.f), e = ex2_ftz(d);
+    s4[k & 3] += e;
+    t4[k & 3] = fmaf(e, d, t4[k & 3]);
   }
+  T.s += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+  T.t += (t4[0] + t4[1]) + (t4[2] + t4[3]);
 }
 
 __device__ lp_key_t lp_block_max(LpShared& S, lp_key_t k) {
@@ -162,37 +163,43 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
   const int id = rank == 0 && tid == 0 && J.ids ? J.ids[r] : -1;
   const float x_id = id >= 0 && id < J.n ? x[id] : 0.f;
 
-  LpThread T = {{-INFINITY, 0.f, 0.f}, -INFINITY, -INFINITY, 0, 0};
-  if (tid < head) {
-    float w[1] = {x[lo + tid]};
-    lp_add<1>(T, w, LP_HEAD, 0, temp, c);
+  LpWarp T = {-INFINITY, 0.f, 0.f, false, -INFINITY};
+  if (warp == 0 && head > 0) {
+    float w[1] = {-INFINITY};
+    if (tid < head) w[0] = lp_clean(x[lo + tid]);
+    lp_add<1>(T, w, c);
   }
   constexpr int UN = 4;  // vectors of a batch, one every LP_THREADS
-  int v = tid;
-  for (; v + (UN - 1) * LP_THREADS < nv; v += UN * LP_THREADS) {
-    float w[4 * UN];
+  int v = tid;           // (the loops' ends are the warp's, not the lane's)
+  for (; v - lane + 31 + (UN - 1) * LP_THREADS < nv; v += UN * LP_THREADS) {
+    float w[UN][4];
 #pragma unroll
-    for (int k = 0; k < UN; ++k) *reinterpret_cast<float4*>(w + 4 * k) = __ldg(xv + v + k * LP_THREADS);
-    lp_add<4 * UN>(T, w, v, UN, temp, c);
+    for (int k = 0; k < UN; ++k) *reinterpret_cast<float4*>(w[k]) = __ldg(xv + v + k * LP_THREADS);
+#pragma unroll
+    for (int k = 0; k < UN; ++k) lp_clean<4>(w[k]);
+    lp_add<4 * UN>(T, reinterpret_cast<float(&)[4 * UN]>(w), c);
   }
-  for (; v < nv; v += LP_THREADS) {
-    float w[4];
-    *reinterpret_cast<float4*>(w) = __ldg(xv + v);
-    lp_add<4>(T, w, v, 1, temp, c);
+  for (; v - lane < nv; v += LP_THREADS) {
+    float w[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+    if (v < nv) {
+      *reinterpret_cast<float4*>(w) = __ldg(xv + v);
+      lp_clean<4>(w);
+    }
+    lp_add<4>(T, w, c);
   }
-  if (tid < tail) {
-    float w[1] = {x[v0 + 4 * nv + tid]};
-    lp_add<1>(T, w, LP_TAIL, 0, temp, c);
+  if (warp == 0 && tail > 0) {
+    float w[1] = {-INFINITY};
+    if (tid < tail) w[0] = lp_clean(x[v0 + 4 * nv + tid]);
+    lp_add<1>(T, w, c);
   }
 
   // ---- sums of the CTA's part
-  LpSums a = T.a;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    a = lp_join(a, {__shfl_down_sync(0xffffffffu, a.m, o), __shfl_down_sync(0xffffffffu, a.s, o),
-                    __shfl_down_sync(0xffffffffu, a.t, o)}, c);
-  if (lane == 0) S.sums[warp] = a;
-  const uint32_t my_z = T.z == -INFINITY ? 0u : ordered_key(T.z);  // 0: no token
+  {
+    const float ws = warp_sum(T.s), wt = warp_sum(T.t);
+    if (lane == 0) S.sums[warp] = {T.m, ws, wt};
+  }
+  const float my_top = lp_z(T.top, temp);
+  const uint32_t my_z = T.top == -INFINITY ? 0u : ordered_key(my_top);  // 0: no token
   if (J.top > 0) {
     uint32_t g = my_z;
 #pragma unroll
@@ -205,7 +212,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
   }
   __syncthreads();
   if (warp == 0) {
-    a = lane < LP_WARPS ? S.sums[lane] : LpSums{-INFINITY, 0.f, 0.f};
+    LpSums a = lane < LP_WARPS ? S.sums[lane] : LpSums{-INFINITY, 0.f, 0.f};
 #pragma unroll
     for (int o = LP_WARPS / 2; o > 0; o >>= 1)
       a = lp_join(a, {__shfl_down_sync(0xffffffffu, a.m, o), __shfl_down_sync(0xffffffffu, a.s, o),
@@ -246,18 +253,17 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
     if (S.over > 0) {  // (uniform) of the groups that share it, those with the lowest indices
       lp_key_t g = 0ull;
       if (my_z == S.kz && S.gz[tid / LP_LANES] == S.kz) {
-        int i = T.at == LP_HEAD ? lo + tid : v0 + 4 * nv + tid;
-        if (T.at >= 0) {
-          i = INT_MAX;
-          for (int q = 0; q < T.vecs; ++q) {
-            const float4 w = __ldg(xv + T.at + q * LP_THREADS);
-            const float e[4] = {w.x, w.y, w.z, w.w};
+        // the thread's first token with its best z
+        int i = tid < head && lp_z(lp_clean(x[lo + tid]), temp) == my_top ? lo + tid : INT_MAX;
+        for (int q = tid; q < nv && i == INT_MAX; q += LP_THREADS) {
+          const float4 w = __ldg(xv + q);
+          const float e[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (lp_z(lp_clean(e[j]), temp) == T.z) i = min(i, v0 + 4 * (T.at + q * LP_THREADS) + j);
-          }
+          for (int j = 3; j >= 0; --j)
+            if (lp_z(lp_clean(e[j]), temp) == my_top) i = v0 + 4 * q + j;
         }
-        g = lp_key(T.z, i);
+        if (i == INT_MAX) i = v0 + 4 * nv + tid;
+        g = lp_key(my_top, i);
       }
 #pragma unroll
       for (int o = LP_LANES / 2; o > 0; o >>= 1) g = max(g, __shfl_xor_sync(0xffffffffu, g, o));
