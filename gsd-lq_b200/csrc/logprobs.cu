@@ -29,6 +29,10 @@ namespace gsdlq {
 // (z, lowest index first) with z as the sampler rounds it, so equal z (different logits can share one) go by index;
 // the tokens' indices are looked up only where the k-th maximum is shared by more groups than are wanted, as in
 // rows with fewer unmasked tokens than k.
+//
+// 128 rows of 151936 (78 MB): 18.4 us without alternatives, 25.6 with 20; 592 rows: 61 us (5.9 TB/s) and 81.  Large
+// batches are bound by HBM, 128 rows by the start and the end of 256 CTAs that all run at once; the alternatives
+// cost a tail of barriers, a second look at 2 % of the tokens and the joining of the cluster's lists.
 constexpr int LP_THREADS = 512, LP_WARPS = LP_THREADS / 32;
 constexpr int LP_LANES = 4, LP_GROUPS = LP_THREADS / LP_LANES;  // groups of neighbouring lanes; >= GSDLQ_MAX_TOP
 constexpr int LP_CAP = 1280;                   // tokens collected before the slow path takes over

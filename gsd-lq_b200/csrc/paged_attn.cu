@@ -20,8 +20,9 @@ namespace gsdlq {
 // that the result does not depend on who that is.
 //
 // Each warp has a K and a V tile of its own (cp.async, no CTA-wide barrier in the loop): the next unit's K is on its
-// way while the weights and the second product are worked on, its V during the next first product.  Twelve such
-// warps an SM keep more bytes in flight and more instructions to choose from than eight with three tiles each.
+// way while the weights and the second product are worked on, its V during the next first product.  Two CTAs an SM
+// keep up to 128 KB on their way; three (at 168 registers a thread, with spills) were slower: 74 us against 63 for 64
+// rows of 1 to 8191 positions.
 //
 // Both products run on mma.m16n8k16 with the 16-bit cache values as they are, so K and V go from shared
 // memory to the matrix unit without a conversion.  q and the weights p are fp32 and enter as parts of 16 bits:
@@ -29,13 +30,21 @@ namespace gsdlq {
 //   bf16: hi + mid + lo, 24 bits: hi and mid in the two halves of one A, lo in the lower half of another
 // so that one product gives both parts and c[0] + c[2], c[1] + c[3] are the sums.  With A = q, B = K^T the score
 // fragment is already p's A fragment for the second product, B = V.  The second product starts from zero each
-// unit and is added to fp32 registers, which keeps the tensor core's truncating accumulation short.
+// unit and is added to fp32 registers, which keeps the tensor core's truncating accumulation short.  (A tile of
+// tcgen05.mma has 128 rows; eight columns in two parts would fill an eighth of it, and at 13-31 % of its cycles the
+// tensor pipe bounds nothing here.)
+//
+// Bound by HBM.  Measured on one B200 (device time, L2 cold): 16 rows x 32 kv heads of 64 over 1025-2047 positions,
+// fp16: 41 us for 195 MB (4.8 TB/s; 5.9 TB/s from the first tile to the last, then 3-4 us of joining); 64 rows x 8 kv
+// heads of 128 over 1-8191 positions, bf16: 54 us for 250 MB; one row x 8 kv heads of 128 over 1537 positions: 9.5 us,
+// of which 2.6 pass before the first tile (positions, table, tile: three dependent look-ups) and 3.5 in the join.
 constexpr int PA_MAX_CTAS = 320;  // largest grid of an attention launch
 constexpr int PA_PER_SM = 2;
 constexpr int PA_GROUP = 8;       // query heads of one kv head taken together
 constexpr int PA_WARPS = 4, PA_THREADS = PA_WARPS * 32;
 constexpr int PA_SHORT = 4;       // units of an item that one warp may take
 // units that an item counts besides its own, for its queries, and for the merge of the warps where it has one
+// (64 rows of 1-8191 positions: 1 and 2 units 62 us, 1 and 4 58, 2 and 4 54, 3 and 5 53, 4 and 6 55)
 __host__ __device__ constexpr int pa_over(int tiles) { return tiles <= PA_SHORT ? 2 : 4; }
 
 constexpr int pa_tok(int hd) { return hd == 128 ? 32 : 64; }  // positions of a unit
@@ -642,8 +651,10 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
 // row.  A pack is a run of rows with the same sequence inside PA_WARPS * rows_warp rows from a multiple of that
 // on, so that every CTA finds the same packs from a row's neighbours alone.  The units are the tiles up to the
 // longest row's end, dealt to the CTAs as above; a warp passes over those that lie behind all its rows.
+// 128 rows at positions 1024-1151 of one sequence, 12 query and 2 kv heads of 128: 25 us (28 without sharing); bound by
+// the latency of a warp's dependent instructions (issue slots 28 % used, tensor pipe 22 % of active cycles).
 constexpr int PC_STAGES = 4;  // tiles of K and V on their way or in use
-constexpr int PC_OVER = 2;    // units that an item counts besides its own
+constexpr int PC_OVER = 2;    // units that an item counts besides its own (those 128 rows: 0 26.8 us, 1 25.7, 4 26.2)
 
 template <int HD>
 struct PagedChunkSmem {
