@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(256) pages_renumber_kernel(const __grid_consta
 // read and written for 448 pages of 28 layers x 2 x 8 KB, 6.6 TB/s for 32 pages of 32 layers x 2 x 32 KB (some of it
 // from L2).
 constexpr int COPY_THREADS = 128, COPY_PER = 4, COPY_PIECE = COPY_THREADS * COPY_PER;
-constexpr int COPY_PER_SM = 16;
+constexpr int COPY_PER_SM = 8;
 struct CopyPlan {
   unsigned words;                   // of a plane of a page
   unsigned pieces, per_pair;        // of a plane; of a page

@@ -259,9 +259,14 @@ struct PaColumns {
 };
 __device__ __forceinline__ float pa_inverse(float x) { return x > 0.f ? 1.f / x : (x == 0.f ? 0.f : NAN); }  // 0: no position left
 
-// Four values (the e-th four of column c) of an item that n_parts CTAs from `first` on hold: a CTA's part lies in its
-// second place where the item begins, else in the first.  A place: [PA_GROUP][HD] weighted sums, then the columns'
-// (maximum, sum of weights); places are `slot` floats apart.
+// Joining the parts of an item that n_parts CTAs from `first` on hold.  A CTA's part lies in its second place where the
+// item begins, else in the first; places are `slot` floats apart.  A place: [PA_GROUP][HD] weighted sums, then the
+// columns' (maximum, sum of weights).  The joining warps are alone on their SM, so what counts is how many loads are in
+// flight and how few instructions follow one another: one load after the other, joining 13 parts took 7 us; it takes 2.
+__device__ __forceinline__ const float* pa_place(const float* part, size_t slot, int first, int i) {
+  return part + ((size_t)(first + i) * 2 + (i == 0)) * slot;
+}
+// A thread's four values of column c (the e-th four), with its own sums of the weights.
 template <int HD>
 __device__ __forceinline__ float4 pa_join(const float* part, size_t slot, int first, int n_parts, int c, int e) {
   constexpr int BATCH = 8;  // parts whose loads are in flight together
@@ -272,8 +277,7 @@ __device__ __forceinline__ float4 pa_join(const float* part, size_t slot, int fi
     float2 ml[BATCH];
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
-      const int q = min(i0 + i, n_parts - 1);
-      const float* const at = part + ((size_t)(first + q) * 2 + (q == 0)) * slot;
+      const float* const at = pa_place(part, slot, first, min(i0 + i, n_parts - 1));
       o[i] = __ldcg(reinterpret_cast<const float4*>(at + c * HD) + e);
       ml[i] = __ldcg(reinterpret_cast<const float2*>(at + PA_GROUP * HD) + c);
       if (i0 + i >= n_parts) ml[i].x = -INFINITY;
@@ -294,6 +298,54 @@ __device__ __forceinline__ float4 pa_join(const float* part, size_t slot, int fi
   }
   const float inv = pa_inverse(L);
   return make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
+}
+// For many values a thread: the parts' factors once per column, then the sums.
+// factors f[i] of a column over the lanes `lane`, `lane + lanes`, ... of those that share it (xor distances from..16)
+template <int HD>
+__device__ __forceinline__ void pa_factors(float* f, const float* part, size_t slot, int first, int n_parts, int c, int i0,
+                                           int lanes) {
+  float M = -INFINITY, L = 0.f;
+  for (int i = i0; i < n_parts; i += lanes) {
+    const float2 ml = __ldcg(reinterpret_cast<const float2*>(pa_place(part, slot, first, i) + PA_GROUP * HD) + c);
+    f[i] = ml.x;
+    const float top = fmaxf(M, ml.x), ref = top == -INFINITY ? 0.f : top;
+    L = fmaf(L, ex2_ftz(M - ref), ml.y * ex2_ftz(ml.x - ref));
+    M = top;
+  }
+  for (int o = 32 / lanes; o < 32; o <<= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, M, o), l2 = __shfl_xor_sync(0xffffffffu, L, o);
+    const float top = fmaxf(M, m2), ref = top == -INFINITY ? 0.f : top;
+    L = fmaf(L, ex2_ftz(M - ref), l2 * ex2_ftz(m2 - ref));
+    M = top;
+  }
+  const float ref = M == -INFINITY ? 0.f : M, inv = pa_inverse(L);
+  for (int i = i0; i < n_parts; i += lanes) f[i] = ex2_ftz(f[i] - ref) * inv;
+}
+// fours e0, e0 + step, .. of the item's columns: the parts' sums times their factors (f: a row of `f_row` per column)
+template <int HD, int E, int BATCH>
+__device__ __forceinline__ void pa_sums(float4 (&A)[E], const float* f, int f_row, const float* part, size_t slot,
+                                        int first, int n_parts, int e0, int step) {
+#pragma unroll
+  for (int k = 0; k < E; ++k) A[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n_parts; i0 += BATCH) {
+    float4 o[BATCH][E];
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const float4* const at = reinterpret_cast<const float4*>(pa_place(part, slot, first, min(i0 + i, n_parts - 1))) + e0;
+#pragma unroll
+      for (int k = 0; k < E; ++k) o[i][k] = __ldcg(at + k * step);
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const float* const fk = f + (e0 + k * step) / (HD / 4) * f_row + i0;
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const float x = i0 + i < n_parts ? fk[i] : 0.f;
+        A[k] = make_float4(fmaf(o[i][k].x, x, A[k].x), fmaf(o[i][k].y, x, A[k].y), fmaf(o[i][k].z, x, A[k].z),
+                           fmaf(o[i][k].w, x, A[k].w));
+      }
+    }
+  }
 }
 
 // a walk over a CTA's run, segment by segment: the part of an item that lies in it
@@ -660,6 +712,7 @@ template <int HD>
 struct PagedChunkSmem {
   uint8_t tile[PC_STAGES][2][pa_tok(HD) * HD * 2];  // K, V
   unsigned valid[PC_STAGES][PA_WARPS];              // of the positions that a warp has looked up
+  float f[PA_WARPS][PA_GROUP][PA_MAX_CTAS];         // the parts' factors, while they are joined
   int seq[PA_THREADS], len[PA_THREADS];             // of the rows, while the packs are counted
   int warp_sum[PA_WARPS];
   int row, base, last;
@@ -947,11 +1000,19 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     __syncthreads();
     if (S.last) {
       __threadfence();
-      for (int e = lane; e < PA_GROUP * HD / 4; e += 32) {
-        const int c = e / (HD / 4), cr = c / gq_max, ch = c - cr * gq_max, r = warp * rows_warp + cr;
-        if (cr < rows_warp && ch < gq && r < n)
-          *(reinterpret_cast<float4*>(J.out + ((size_t)(row + r) * J.n_heads + head0 + ch) * HD) + e % (HD / 4)) =
-              pa_join<HD>(part, PLACE, first, n_parts, c, e % (HD / 4));
+      constexpr int E = HD == 32 ? 2 : 4;
+      const int columns = min(PA_GROUP, rows_warp * gq_max);  // (what columns of no row hold is not looked at)
+      pa_factors<HD>(S.f[warp][lane & 7], part, PLACE, first, n_parts, lane & 7, lane >> 3, 4);
+      __syncwarp();
+      for (int e0 = lane; e0 < columns * (HD / 4); e0 += 32 * E) {
+        float4 A[E];
+        pa_sums<HD, E, 6>(A, S.f[warp][0], PA_MAX_CTAS, part, PLACE, first, n_parts, e0, 32);
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+          const int e = e0 + 32 * k, c = e / (HD / 4), cr = c / gq_max, ch = c - cr * gq_max, r = warp * rows_warp + cr;
+          if (c < columns && ch < gq && r < n)
+            *(reinterpret_cast<float4*>(J.out + ((size_t)(row + r) * J.n_heads + head0 + ch) * HD) + e % (HD / 4)) = A[k];
+        }
       }
       if (tid == 0) *count = 0u;
     }
