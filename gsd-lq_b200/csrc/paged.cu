@@ -354,9 +354,9 @@ __global__ void __launch_bounds__(256) pages_renumber_kernel(const __grid_consta
 }
 
 // Pages: copy.  The planes (layer, K or V) of the pairs' pages are cut into pieces of at most COPY_PIECE 16-byte
-// words, dealt to the CTAs in turn; the next piece's pair is looked up while a piece is copied.  Bound by HBM: 5.7 TB/s
-// read and written for 448 pages of 28 layers x 2 x 8 KB, 6.6 TB/s for 32 pages of 32 layers x 2 x 32 KB (some of it
-// from L2).
+// words, dealt to the CTAs in turn; the next piece's pair is looked up while a piece is copied.  Bound by HBM: 5.8 TB/s
+// read and written for 448 pages of 28 layers x 2 x 8 KB, 6.9 TB/s for 32 pages of 32 layers x 2 x 32 KB (some of it
+// from L2); other shapes of the pieces and 16 CTAs an SM are within 3 %.
 constexpr int COPY_THREADS = 128, COPY_PER = 4, COPY_PIECE = COPY_THREADS * COPY_PER;
 constexpr int COPY_PER_SM = 8;
 struct CopyPlan {

@@ -52,7 +52,7 @@ constexpr int pa_tok(int hd) { return hd == 128 ? 32 : 64; }  // positions of a 
 template <int HD>
 struct PagedAttnSmem {
   uint8_t tile[PA_WARPS][2][pa_tok(HD) * HD * 2];  // K, V
-  float acc[PA_WARPS][PA_GROUP][HD < 64 ? HD : 64];  // the warps' results of an item, 64 dimensions at a time
+  float acc[PA_WARPS][PA_GROUP][HD];               // the warps' results of an item
   float m[PA_WARPS][PA_GROUP], l[PA_WARPS][PA_GROUP];
   int warp_sum[PA_WARPS];
   int row, base, last;
@@ -258,6 +258,15 @@ struct PaColumns {
   }
 };
 __device__ __forceinline__ float pa_inverse(float x) { return x > 0.f ? 1.f / x : (x == 0.f ? 0.f : NAN); }  // 0: no position left
+
+// One thread, after a barrier behind which the CTA's part is written: whether it is the last of n_parts CTAs, whose
+// parts the CTA may then read, after another barrier.
+__device__ __forceinline__ bool pa_arrive(unsigned* count, int n_parts) {
+  __threadfence();
+  const bool last = atomicAdd(count, 1u) == (unsigned)n_parts - 1u;
+  if (last) __threadfence();
+  return last;
+}
 
 // Joining the parts of an item that n_parts CTAs from `first` on hold.  A CTA's part lies in its second place where the
 // item begins, else in the first; places are `slot` floats apart.  A place: [PA_GROUP][HD] weighted sums, then the
@@ -637,54 +646,45 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     const int first = cur.s / per, n_parts = (cur.s + cur.tiles - 1) / per - first + 1;  // CTAs that hold the item
     float* const mine = part + ((size_t)cta * 2 + (cur.s >= v0)) * PA_GROUP * (HD + 2);
     unsigned* const count = static_cast<unsigned*>(J.work) + (size_t)cur.row * items_row + cur.item;
-    constexpr int DIMS = HD < 64 ? HD : 64;
+    if (h < gq) {
 #pragma unroll
-    for (int d0 = 0; d0 < HD; d0 += DIMS) {
-      if (d0 > 0) __syncthreads();  // the first dimensions are merged
-      if (h < gq) {
-#pragma unroll
-        for (int n = 0; n < DIMS / 8; ++n)
-          *reinterpret_cast<float2*>(&S.acc[warp][h][n * 8 + 2 * (lane & 3)]) =
-              make_float2(C.acc[d0 / 8 + n][0], C.acc[d0 / 8 + n][1]);
-        if (d0 == 0 && (lane & 3) == 0) {
-          S.m[warp][h] = C.m * C.scale;
-          S.l[warp][h] = C.l;
-        }
+      for (int n = 0; n < CH; ++n)
+        *reinterpret_cast<float2*>(&S.acc[warp][h][n * 8 + 2 * (lane & 3)]) = make_float2(C.acc[n][0], C.acc[n][1]);
+      if ((lane & 3) == 0) {
+        S.m[warp][h] = C.m * C.scale;
+        S.l[warp][h] = C.l;
       }
-      if (d0 + DIMS == HD) have = next_seg();
-      __syncthreads();
-      for (int e = tid; e < gq * DIMS / 4; e += PA_THREADS) {
-        const int hh = e / (DIMS / 4), d = e % (DIMS / 4) * 4;
-        float M = S.m[0][hh];
+    }
+    have = next_seg();
+    __syncthreads();
+    for (int e = tid; e < gq * HD / 4; e += PA_THREADS) {
+      const int hh = e / (HD / 4), d = e % (HD / 4) * 4;
+      float M = S.m[0][hh];
 #pragma unroll
-        for (int w = 1; w < PA_WARPS; ++w) M = fmaxf(M, S.m[w][hh]);
-        const float ref = M == -INFINITY ? 0.f : M;
-        float L = 0.f;
-        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int w = 1; w < PA_WARPS; ++w) M = fmaxf(M, S.m[w][hh]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      float L = 0.f;
+      float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < PA_WARPS; ++w) {
-          const float f = ex2_ftz(S.m[w][hh] - ref);
-          const float4 o = *reinterpret_cast<const float4*>(&S.acc[w][hh][d]);
-          L = fmaf(S.l[w][hh], f, L);
-          A = make_float4(fmaf(o.x, f, A.x), fmaf(o.y, f, A.y), fmaf(o.z, f, A.z), fmaf(o.w, f, A.w));
-        }
-        if (whole) {
-          const float inv = pa_inverse(L);
-          *reinterpret_cast<float4*>(out + hh * HD + d0 + d) = make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
-        } else {
-          __stcg(reinterpret_cast<float4*>(mine + hh * HD + d0 + d), A);
-          if (d0 + d == 0) __stcg(reinterpret_cast<float2*>(mine + PA_GROUP * HD) + hh, make_float2(M, L));
-        }
+      for (int w = 0; w < PA_WARPS; ++w) {
+        const float f = ex2_ftz(S.m[w][hh] - ref);
+        const float4 o = *reinterpret_cast<const float4*>(&S.acc[w][hh][d]);
+        L = fmaf(S.l[w][hh], f, L);
+        A = make_float4(fmaf(o.x, f, A.x), fmaf(o.y, f, A.y), fmaf(o.z, f, A.z), fmaf(o.w, f, A.w));
+      }
+      if (whole) {
+        const float inv = pa_inverse(L);
+        *reinterpret_cast<float4*>(out + hh * HD + d) = make_float4(A.x * inv, A.y * inv, A.z * inv, A.w * inv);
+      } else {
+        __stcg(reinterpret_cast<float4*>(mine + hh * HD + d), A);
+        if (d == 0) __stcg(reinterpret_cast<float2*>(mine + PA_GROUP * HD) + hh, make_float2(M, L));
       }
     }
     if (!whole) {
-      // an item's part lies in its CTA's second place where it begins, else in the first
-      __threadfence();
       __syncthreads();
-      if (tid == 0) S.last = atomicAdd(count, 1u) == (unsigned)n_parts - 1u;
+      if (tid == 0) S.last = pa_arrive(count, n_parts);
       __syncthreads();
       if (S.last) {
-        __threadfence();
         for (int e = tid; e < gq * HD / 4; e += PA_THREADS)
           *(reinterpret_cast<float4*>(out) + e) =
               pa_join<HD>(part, PA_GROUP * (HD + 2), first, n_parts, e / (HD / 4), e % (HD / 4));
@@ -703,10 +703,11 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
 // row.  A pack is a run of rows with the same sequence inside PA_WARPS * rows_warp rows from a multiple of that
 // on, so that every CTA finds the same packs from a row's neighbours alone.  The units are the tiles up to the
 // longest row's end, dealt to the CTAs as above; a warp passes over those that lie behind all its rows.
-// 128 rows at positions 1024-1151 of one sequence, 12 query and 2 kv heads of 128: 25 us (28 without sharing); bound by
+// 128 rows at positions 1024-1151 of one sequence, 12 query and 2 kv heads of 128: 23 us (28 without sharing), of which
+// 5 pass before the first tile, 9.5 in eight units a CTA and 5 in writing and joining the parts; the units are bound by
 // the latency of a warp's dependent instructions (issue slots 28 % used, tensor pipe 22 % of active cycles).
 constexpr int PC_STAGES = 4;  // tiles of K and V on their way or in use
-constexpr int PC_OVER = 2;    // units that an item counts besides its own (those 128 rows: 0 26.8 us, 1 25.7, 4 26.2)
+constexpr int PC_OVER = 2;    // units that an item counts besides its own (those 128 rows: 0 26.8 us, 1 25.7, 2 24.9, 4 26.2)
 
 template <int HD>
 struct PagedChunkSmem {
@@ -994,12 +995,10 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     unsigned* const count = static_cast<unsigned*>(J.work) + (size_t)cur.row * items_row + cur.item;
     const int row = cur.row, n = cur.n;
     have = next_seg();
-    __threadfence();
     __syncthreads();
-    if (tid == 0) S.last = atomicAdd(count, 1u) == (unsigned)n_parts - 1u;
+    if (tid == 0) S.last = pa_arrive(count, n_parts);
     __syncthreads();
     if (S.last) {
-      __threadfence();
       constexpr int E = HD == 32 ? 2 : 4;
       const int columns = min(PA_GROUP, rows_warp * gq_max);  // (what columns of no row hold is not looked at)
       pa_factors<HD>(S.f[warp][lane & 7], part, PLACE, first, n_parts, lane & 7, lane >> 3, 4);
