@@ -423,6 +423,9 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     if (paged_row(kv, J.row_seq, J.pos, r, false).len == 0)
       for (int i = tid; i < J.n_heads * HD; i += PA_THREADS) J.out[(size_t)r * J.n_heads * HD + i] = 0.f;
   if (v0 >= v1) return;
+  // (the row is found unless the positions change meanwhile, which ends in no row and no wait)
+  if (tid == 0) S.row = -1;
+  __syncthreads();
   if (J.rows <= PA_THREADS) {
     if (base0 <= v0 && v0 < base0 + mine0) {
       S.row = tid;
@@ -430,7 +433,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     }
   } else {
     int before = 0;
-    for (int r0 = 0; before <= v0; r0 += PA_THREADS) {  // (ends: v0 < units)
+    for (int r0 = 0; r0 < J.rows && before <= v0; r0 += PA_THREADS) {
       const int r = r0 + tid, n = r < J.rows ? row_units(paged_row(kv, J.row_seq, J.pos, r, false).len) : 0;
       int total;
       __syncthreads();  // the previous sums are read
@@ -443,6 +446,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     }
   }
   __syncthreads();
+  if (S.row < 0) return;
 
   auto enter = [&](PagedWalk& w, int row) {
     const PagedRow pr = paged_row(kv, J.row_seq, J.pos, row, false);
@@ -798,8 +802,10 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     if (paged_row(kv, J.row_seq, J.pos, r, false).len == 0)
       for (int i = tid; i < J.n_heads * HD; i += PA_THREADS) J.out[(size_t)r * J.n_heads * HD + i] = 0.f;
   if (v0 >= v1) return;
+  if (tid == 0) S.row = -1;  // as above
+  __syncthreads();
   int before = 0;
-  for (int r0 = 0; before <= v0; r0 += PA_THREADS) {  // (ends: v0 < units)
+  for (int r0 = 0; r0 < J.rows && before <= v0; r0 += PA_THREADS) {
     int n = n0, b = base0, total = 0;
     if (J.rows > PA_THREADS) {
       n = pack_units(r0, false);
@@ -814,6 +820,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     before += total;
   }
   __syncthreads();
+  if (S.row < 0) return;
 
   auto enter = [&](PagedPack& w, int row) {  // the pack that begins with `row`
     const int r = row + lane;
