@@ -701,7 +701,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
 }
 
 // ---------------------------------------------------------------------------------------
-// Rows that share sequences (chunks of prompts, several drafted tokens): an item is a pack of neighbouring rows of
+// Rows that share sequences (chunks of prompts, drafted tokens of many sequences): an item is a pack of neighbouring rows of
 // one sequence and a kv head.  The CTA's warps share the tiles of K and V, and each has rows of its own: as many as
 // fill its eight columns.  So a tile is fetched once for up to 32 rows, where the kernel above fetches it for every
 // row.  A pack is a run of rows with the same sequence inside PA_WARPS * rows_warp rows from a multiple of that
@@ -1047,9 +1047,14 @@ static int launch_attention_paged(const gsdlq_paged_attn_job_t& J, int subs, cud
   }
   const int grid = std::min(PA_PER_SM * num_sms(), PA_MAX_CTAS);
   const int ps = J.kv.page_size, shift = ps & (ps - 1) ? -1 : __builtin_ctz((unsigned)ps);
-  // rows share sequences on average: the tiles are worth sharing too
-  if (J.row_seq != nullptr && J.rows >= 2 * J.kv.n_seqs) {
-    const int gq = J.n_heads / J.kv.n_kv_heads;
+  // Several rows a sequence on average, and enough of them: the tiles are worth sharing.  A CTA's warps without rows
+  // are idle then, and its start and end take 4-5 us more.  One tile per row against shared tiles, us:
+  //   16 sequences of 1500, 32/32 heads of 64: 2 rows each 62 / 73, 3 rows 83 / 76; 32/8 of 128: 3 rows 51 / 49, 8 rows
+  //   99 / 45; 12/2 of 128: 3 rows 18.7 / 22.9, 4 rows 23.4 / 22.3; 16/2 of 64: 3 rows 13.5 / 15.9, 4 rows 15.6 / 15.3
+  //   one sequence of 1500, 32/32 of 64: 4 rows 14.9 / 13.4; 32/8 of 128: 8 rows 15.3 / 18.9, 16 rows 20.9 / 20.2;
+  //   12/2 of 128: 32 rows 16.6 / 19.6, 128 rows 28 / 23
+  const int gq = J.n_heads / J.kv.n_kv_heads;
+  if (J.row_seq != nullptr && J.rows >= (gq <= 4 ? 3 : 4) * J.kv.n_seqs && (long long)J.rows * J.kv.n_kv_heads >= 128) {
     const int rows_warp = gq == 1 ? 8 : gq == 2 ? 4 : gq <= 4 ? 2 : 1;  // rows whose heads fill a warp's columns
     return launch_pdl(attention_paged_chunk_kernel<HD, BF16>, grid, PA_THREADS, smem_chunk, st, 1, J, subs, shift, rows_warp);
   }

@@ -195,6 +195,27 @@ def test_attention_leaves_out_missing_pages(cuda_lib, rng):
     assert set(flags()) == {"bad_page", "bad_pos"}
 
 
+def test_attention_of_chunks_leaves_out_missing_pages(cuda_lib, rng):
+    """The same where enough rows share sequences to share tiles."""
+    kv = make_pool(rng, [64, 64, 16], 16, 4, 64, torch.float16)
+    k, v = rows_of(kv, 0, 0, 64)
+    k2, v2 = rows_of(kv, 0, 2, 16)
+    keep = np.r_[0:16, 32:64]
+    kv.table[0, 1] = -1
+    kv.table[1] = torch.tensor([kv.n_pages, -7, 1 << 30, -(1 << 31)] + [-1] * (kv.max_blocks - 4), dtype=torch.int32)
+    rows = [(0, 63), (0, 62), (1, 63), (1, 5), (2, 15), (2, 3), (0, -2), (0, kv.max_blocks * 16), (3, 2), (-1, 2)] * 4
+    q = torch.from_numpy(rng.standard_normal((len(rows), 4, 64))).float().cuda()
+    got = run_attention(kv, 0, q, [p for _, p in rows], [s for s, _ in rows])
+    for r, (s, p) in enumerate(rows):
+        if s in (1, 3, -1) or p not in range(64):
+            assert not got[r].any()
+            continue
+        n = keep[keep <= p] if s == 0 else np.arange(p + 1)
+        want, tol = O.attention(q[r].cpu().numpy(), (k if s == 0 else k2)[n], (v if s == 0 else v2)[n], 0.125)
+        assert (np.abs(got[r] - want) <= tol).all(), r
+    assert set(flags()) == {"bad_page", "bad_pos"}
+
+
 def test_attention_offsets_past_32_bits(cuda_lib, rng):
     """Pages whose elements lie more than 2^32 behind the start of the pool."""
     from gsdlq_b200 import paged
