@@ -137,6 +137,14 @@ def test_tensors_off_the_gpu_are_refused():
         ops.logprobs_job([[0.0]], entropy=torch.zeros(1))
 
 
+def test_launches_stay_on_the_current_device(monkeypatch):
+    """A launch goes to the current device's stream, so tensors on another device are refused."""
+    from gsdlq_b200 import ops
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    with pytest.raises(ValueError, match="cuda:0 is the current device"):
+        ops._stream_on(torch.device("cuda", 1))
+
+
 def test_struct_sizes_match_the_header(tmp_path):
     """The ctypes structs have the C structs' sizes."""
     import os
