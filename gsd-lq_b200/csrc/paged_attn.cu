@@ -58,15 +58,19 @@ struct PagedAttnSmem {
   int row, base, last;
 };
 
-inline size_t attention_paged_counters(int rows, int n_heads, int n_kv) {
+// The work area: two partial results per CTA (its first and its last item), in the form for rows that share sequences
+// one per warp, then the items' counters, which are zero between launches.  The results' part has the same size for
+// every launch, whatever its rows, heads and head size are, so none ever writes where another one counts, and one area
+// serves launches of any shapes in turn.
+constexpr size_t PA_PARTS = sizeof(float) * (size_t)PA_MAX_CTAS * 2 * PA_WARPS * PA_GROUP * (128 + 2);
+static_assert(PA_PARTS % 16 == 0, "the counters follow");
+inline size_t attention_paged_work(int rows, int n_heads, int n_kv) {
   const size_t items = (size_t)rows * n_kv * ((n_heads / n_kv + PA_GROUP - 1) / PA_GROUP);
-  return (items * sizeof(unsigned) + 15) / 16 * 16;
+  return PA_PARTS + (items * sizeof(unsigned) + 15) / 16 * 16;
 }
-// counters of the items, then two partial results per CTA (its first and its last item), in the form for rows that
-// share sequences one per warp
-inline size_t attention_paged_work(int rows, int n_heads, int n_kv, int hd) {
-  return attention_paged_counters(rows, n_heads, n_kv) +
-         sizeof(float) * (size_t)PA_MAX_CTAS * 2 * PA_WARPS * PA_GROUP * (hd + 2);
+__device__ __forceinline__ float* pa_parts(void* work) { return static_cast<float*>(work); }
+__device__ __forceinline__ unsigned* pa_counter(void* work, size_t item) {
+  return reinterpret_cast<unsigned*>(static_cast<uint8_t*>(work) + PA_PARTS) + item;
 }
 
 template <bool BF16>
@@ -598,8 +602,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
   look(U);
   bool have = next_seg();
 
-  float* const part = reinterpret_cast<float*>(static_cast<uint8_t*>(J.work) +
-                                               ((size_t)J.rows * items_row * sizeof(unsigned) + 15) / 16 * 16);
+  float* const part = pa_parts(J.work);
   // this lane's rows of the first K and V matrices
   const uint32_t k0 = kt + pa_at<HD>(lane & 7, lane >> 3), vt0 = kt + TILE + pa_at<HD>(lane & 15, lane >> 4);
   while (have) {
@@ -649,7 +652,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     const bool whole = cur.whole();
     const int first = cur.s / per, n_parts = (cur.s + cur.tiles - 1) / per - first + 1;  // CTAs that hold the item
     float* const mine = part + ((size_t)cta * 2 + (cur.s >= v0)) * PA_GROUP * (HD + 2);
-    unsigned* const count = static_cast<unsigned*>(J.work) + (size_t)cur.row * items_row + cur.item;
+    unsigned* const count = pa_counter(J.work, (size_t)cur.row * items_row + cur.item);
     if (h < gq) {
 #pragma unroll
       for (int n = 0; n < CH; ++n)
@@ -941,9 +944,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
   bool have = next_seg();
   int stage = 0;
   constexpr size_t PLACE = (size_t)PA_WARPS * PA_GROUP * (HD + 2);  // floats of a CTA's part
-  float* const part = reinterpret_cast<float*>(static_cast<uint8_t*>(J.work) +
-                                               ((size_t)J.rows * items_row * sizeof(unsigned) + 15) / 16 * 16) +
-                      warp * PA_GROUP * (HD + 2);
+  float* const part = pa_parts(J.work) + warp * PA_GROUP * (HD + 2);
   while (have) {
     C.begin(x, J.sm_scale);
     for (; cur.t < cur.b; ++cur.t) {
@@ -999,7 +1000,7 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
         __stcg(reinterpret_cast<float2*>(place + h * HD + n * 8 + 2 * (lane & 3)), make_float2(C.acc[n][0], C.acc[n][1]));
       if ((lane & 3) == 0) __stcg(reinterpret_cast<float2*>(place + PA_GROUP * HD) + h, make_float2(C.m * C.scale, C.l));
     }
-    unsigned* const count = static_cast<unsigned*>(J.work) + (size_t)cur.row * items_row + cur.item;
+    unsigned* const count = pa_counter(J.work, (size_t)cur.row * items_row + cur.item);
     const int row = cur.row, n = cur.n;
     have = next_seg();
     __syncthreads();
@@ -1070,7 +1071,7 @@ extern "C" {
 int gsdlq_attention_paged_work_size(int rows, int n_heads, int n_kv_heads, int head_dim, size_t* bytes) {
   if (!bytes || rows <= 0 || n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads) return GSDLQ_ERR_INVALID;
   if (head_dim != 32 && head_dim != 64 && head_dim != 128) return GSDLQ_ERR_INVALID;
-  *bytes = attention_paged_work(rows, n_heads, n_kv_heads, head_dim);
+  *bytes = attention_paged_work(rows, n_heads, n_kv_heads);
   return GSDLQ_OK;
 }
 
@@ -1082,7 +1083,7 @@ int gsdlq_attention_paged(const gsdlq_paged_attn_job_t* job, gsdlq_stream_t stre
     return GSDLQ_ERR_INVALID;
   if (!aligned16(J.q) || !aligned16(J.out) || !aligned16(J.work) || J.q_stride % 4) return GSDLQ_ERR_INVALID;
   if (J.q_stride && J.q_stride < J.n_heads * J.kv.head_dim) return GSDLQ_ERR_INVALID;
-  if (J.work_bytes < attention_paged_work(J.rows, J.n_heads, J.kv.n_kv_heads, J.kv.head_dim)) return GSDLQ_ERR_INVALID;
+  if (J.work_bytes < attention_paged_work(J.rows, J.n_heads, J.kv.n_kv_heads)) return GSDLQ_ERR_INVALID;
   const int gq = J.n_heads / J.kv.n_kv_heads, subs = (gq + PA_GROUP - 1) / PA_GROUP;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // units and places of a layer's pool are counted in 31 bits

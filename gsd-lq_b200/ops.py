@@ -354,7 +354,8 @@ def rope_kv_paged(job):
 
 
 def attention_paged_work(kv, rows: int, n_heads: int) -> torch.Tensor:
-    """A zeroed work area for attention_paged of up to ``rows`` rows (one per launch that may overlap)."""
+    """A zeroed work area for attention_paged, shared by any jobs of up to ``rows`` rows that follow one another (one
+    per launch that may overlap)."""
     n = ctypes.c_size_t()
     L.check(_lib().gsdlq_attention_paged_work_size(rows, n_heads, kv.n_kv_heads, kv.head_dim, ctypes.byref(n)),
             "attention_paged_work_size")

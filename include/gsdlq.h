@@ -490,8 +490,10 @@ int gsdlq_rope_kv_paged(const gsdlq_paged_append_job_t *job, gsdlq_stream_t stre
  * (GSDLQ_FLAG_BAD_PAGE); a row with no position left gives zeros.  Cache rows in use and q must be
  * finite; what lies behind pos[r] in a page is never used, whatever it holds.
  * work: gsdlq_attention_paged_work_size bytes, 16-byte aligned, all zero before its first use; each
- * launch leaves it as it needs it.  Launches that may overlap in time (other streams, graphs that run
- * side by side) need a work area each.  GSDLQ_ERR_UNSUPPORTED: n_pages * page_size above 2^31 - 1, or
+ * launch leaves it as the next one needs it, so one area serves launches of different rows, heads and
+ * head sizes in turn, if it has the largest of their sizes (a size grows with rows * n_kv_heads).
+ * Launches that may overlap in time (other streams, graphs that run side by side) need a work area
+ * each.  GSDLQ_ERR_UNSUPPORTED: n_pages * page_size above 2^31 - 1, or
  * rows * n_kv_heads * max_blocks * page_size above about 2^35. */
 typedef struct gsdlq_paged_attn_job {
   gsdlq_paged_kv_t kv;

@@ -148,6 +148,36 @@ def test_attention_chunks_over_long_caches(cuda_lib, rng):
             check_attention(kv, 0, q, pos, [0] * rows)
 
 
+def test_one_work_area_serves_launches_of_any_shape_in_turn(cuda_lib, rng):
+    """Launches of few and many rows, in both forms and of all head sizes, on one work area: each the same bit for bit
+    as with a work area of its own, with every row written, and within the bound."""
+    from gsdlq_b200 import ops, paged
+    shared = None
+    for hd, nkv, group in ((64, 32, 1), (128, 8, 4), (32, 8, 1), (64, 32, 1)):
+        one = make_pool(rng, [1260], 16, nkv, hd, torch.float16)
+        table = torch.full((400, one.max_blocks), -1, dtype=torch.int32, device="cuda")
+        table[0] = one.table[0]
+        many = paged.PagedKV.wrap(one.k, one.v, table, one.refs)  # as many sequences: a tile per row
+        heads = nkv * group
+        if shared is None:
+            shared = ops.attention_paged_work(one, 300, 32)
+        for rows in (30, 128, 6, 128, 2, 64, 300, 1, 128):
+            q = torch.from_numpy(rng.standard_normal((rows, heads, hd)) * 2).float().cuda()
+            pos, seq = [900 + r for r in range(rows)], dev([0] * rows)
+            for kv in (one, many):
+                outs = []
+                for work in (shared, ops.attention_paged_work(kv, rows, heads)):
+                    out = torch.full((rows, heads, hd), math.nan, device="cuda")
+                    ops.attention_paged(ops.paged_attn_job(kv, 0, q, out, dev(pos), hd ** -0.5, work, seq))
+                    outs.append(out.cpu().numpy())
+                assert np.array_equal(outs[0], outs[1]), (hd, rows, kv is one)
+                for r in {0, rows // 2, rows - 1}:
+                    k, v = rows_of(kv, 0, 0, pos[r] + 1)
+                    want, tol = O.attention(q[r].cpu().numpy(), k, v, hd ** -0.5)
+                    assert (np.abs(outs[0][r] - want) <= tol).all(), (hd, rows, r)
+    assert flags() == []
+
+
 def test_attention_strided_q_and_extreme_scores(cuda_lib, rng):
     kv = make_pool(rng, [50, 200, 7], 16, 2, 64, torch.float16)
     wide = torch.from_numpy(rng.standard_normal((3, 4 * 64 + 20))).float().cuda()

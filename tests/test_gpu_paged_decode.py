@@ -72,6 +72,56 @@ def test_paged_decode_matches_the_contiguous_cache(cuda_lib, name, mode, batch, 
     m.release()
 
 
+@pytest.mark.parametrize("batch", [2, 16, 32, 128])
+def test_prompts_between_steps_match_the_contiguous_cache(cuda_lib, batch):
+    """One decoder takes prompts and steps in turn: chunks of 128 rows and fewer and steps of ``batch`` rows follow one
+    another in every order, and each step's logits are those of the contiguous cache."""
+    import gsdlq_b200._lib as L
+    from gsdlq_b200.batch import BatchDecoder
+    from gsdlq_b200.paged import PagedBatchDecoder
+    m, cfg = model("smollm2-1.7b", "turbo", n_layers=2)
+    rng = np.random.default_rng(17)
+    vocab, S = cfg["vocab_size"], 320
+    bd = BatchDecoder(m, batch, max_seq=S)
+    pd = PagedBatchDecoder(m, batch, batch * 20, 16, max_seq=S)
+    at, tok = [0] * batch, rng.integers(0, vocab, batch).tolist()
+
+    def prompt(b, n):
+        ids = rng.integers(0, vocab, n).tolist()
+        for d in (bd, pd):
+            d.prefill(b, ids[:-1])
+        at[b], tok[b] = n - 1, ids[-1]
+
+    def steps(n):
+        for d in (bd, pd):
+            d.set_tokens(tok, at)
+        for _ in range(n):
+            bd.step()
+            pd.step()
+            a, b = bd.logits_host(), pd.logits_host()
+            assert np.abs(a - b).max() < LOGIT_TOL
+            pd.ids.copy_(bd.ids)
+            for s in range(batch):
+                at[s] += 1
+        tok[:] = bd.ids.tolist()
+
+    prompt(0, 150)
+    prompt(1, 300)
+    steps(2)
+    for b, n in ((0, 300), (1, 130), (batch - 1, 290), (0, 3)):
+        pd.free([b])
+        prompt(b, n)
+        steps(2)
+    pd.free(range(batch))
+    for b in range(batch):
+        prompt(b, int(rng.integers(2, 310)))
+    steps(3)
+    assert L.device_flags() == 0
+    bd.release()
+    pd.release()
+    m.release()
+
+
 def test_generate_idle_sequences_and_page_exhaustion(cuda_lib):
     import gsdlq_b200._lib as L
     from gsdlq_b200.paged import PagedBatchDecoder

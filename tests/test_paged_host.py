@@ -177,3 +177,22 @@ def test_restated_page_bookkeeping():
     assert p.refs == [1, 1, 0, 1, 0, 1]
     assert p.compact(1) == ([(5, 2)], 4, 4) and p.table[1][0] == 2
     assert p.compact(9) == ([], 4, 4)
+
+
+def test_attention_work_serves_every_shape_in_turn():
+    """What a launch keeps beside its counters has one size whatever its shape is, so that one area serves launches of
+    any rows, heads and head sizes in turn."""
+    lib = L.load()
+
+    def size(rows, heads, kv_heads, hd):
+        n = ctypes.c_size_t()
+        assert lib.gsdlq_attention_paged_work_size(rows, heads, kv_heads, hd, ctypes.byref(n)) == 0
+        return n.value
+
+    for rows, heads, kv_heads in ((1, 4, 4), (128, 32, 32), (300, 32, 8), (7, 40, 2)):
+        items = rows * kv_heads * -(-heads // kv_heads // 8)  # groups of up to eight heads
+        assert len({size(rows, heads, kv_heads, hd) - -(-items // 4) * 16 for hd in (32, 64, 128)}) == 1
+    parts = {size(rows, heads, kv_heads, hd) - -(-rows * kv_heads // 4) * 16
+             for rows, heads, kv_heads, hd in ((1, 4, 4, 32), (128, 32, 32, 64), (300, 32, 8, 128), (2, 2, 1, 64))}
+    assert len(parts) == 1
+    assert all(size(r, 32, 8, 64) <= size(r + 1, 32, 8, 64) for r in range(1, 70))
