@@ -72,8 +72,14 @@ __device__ __forceinline__ lp_key_t lp_key(float z, int i) {
   return ((lp_key_t)ordered_key(z) << 32) | (0xffffffffu - (uint32_t)i);
 }
 __device__ __forceinline__ int lp_index(lp_key_t k) { return (int)(0xffffffffu - (uint32_t)k); }
-// a little below x: logits that may round to the same z as x lie above it
-__device__ __forceinline__ float lp_below(float x) { return x - fmaf(fabsf(x), 9.5367431640625e-07f, FLT_MIN); }
+// A logit below which no quotient reaches z.  A quotient is z if it lies less than z's own rounding step away (a share
+// of 2^-23, or 2^-149 where z is subnormal), and the product with the temperature rounds too; the quotients at -FLT_MAX
+// include all that lie below it.
+__device__ __forceinline__ float lp_below(float z, float temp) {
+  constexpr float REL = 9.5367431640625e-07f, TINY = 2.8025969e-45f;  // 2^-20; two subnormal steps
+  const float x = (z - fmaf(fabsf(z), REL, TINY)) * temp;             // -inf for z = -FLT_MAX
+  return x - fmaf(fabsf(x), REL, FLT_MIN);
+}
 
 __device__ __forceinline__ LpSums lp_join(LpSums a, LpSums b, float c) {
   const LpSums hi = a.m >= b.m ? a : b, lo = a.m >= b.m ? b : a;
@@ -283,7 +289,7 @@ __global__ void __launch_bounds__(LP_THREADS, 2)
       K = S.K;
     }
     const float zk = K ? key_to_float((uint32_t)(K >> 32)) : -INFINITY;
-    const float close = K ? lp_below(zk * temp) : -INFINITY;
+    const float close = K ? lp_below(zk, temp) : -INFINITY;
     auto look = [&](float v, int i) {
       v = lp_clean(v);
       if (v >= close) {

@@ -549,7 +549,8 @@ int gsdlq_pages_copy(const gsdlq_paged_kv_t *kv, const int *src, const int *dst,
  *   entropy[r]  = -sum_i p_i log p_i (NULL: not computed)
  *   top_ids[r][j], top_logprobs[r][j], j < top: the largest log p in descending order, equal ones by
  *                 ascending index.  0 <= top <= min(n, GSDLQ_MAX_TOP)
- * temperature > 0 and finite.  row_stride: elements between rows, 0: packed. */
+ * temperature > 0 and finite; a quotient past fp32's range counts as its largest value of that sign when
+ * alternatives are ordered (its log p is that value or -inf).  row_stride: elements between rows, 0: packed. */
 #define GSDLQ_MAX_TOP 32
 typedef struct gsdlq_logprobs_job {
   const float *logits;

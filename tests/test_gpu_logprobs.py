@@ -117,6 +117,39 @@ def test_masked_and_non_finite_logits(cuda_lib, rng):
         assert not any(np.isnan(v).any() for v in got.values())
 
 
+@pytest.mark.parametrize("rows,n", [(3, 700), (2, 151936), (200, 4097)])
+def test_alternatives_among_quotients_past_the_range(cuda_lib, rng, rows, n):
+    """Rows with fewer unmasked tokens than alternatives, masked with the type's lowest value or another value whose
+    quotient is past the type's range, count those quotients as -FLT_MAX: equal, in order of their indices."""
+    big = np.float32(np.finfo(np.float32).max)
+    for temp in (0.5, 0.9999, 1e-4, 1.0, 2.0):
+        x = torch.full((rows, n), -float(big), device="cuda")
+        x[:, 5::7] = -float(big) * 0.75
+        for r in range(rows):
+            x[r, torch.from_numpy(rng.permutation(n)[:r % 4])] = torch.from_numpy(
+                rng.standard_normal(r % 4).astype(np.float32)).cuda()
+        got = run(x, list(range(rows)), 20, temp)
+        xs = x.cpu().numpy()
+        with np.errstate(over="ignore"):
+            z = np.clip(xs / np.float32(temp), -big, big)
+        order = np.argsort(-z, axis=1, kind="stable")[:, :20]
+        assert np.array_equal(got["top_ids"], order), temp
+        for r in range(rows):
+            assert np.isfinite(got["top_logprobs"][r, :r % 4]).all()
+            assert (got["top_logprobs"][r, 1:] <= got["top_logprobs"][r, :-1]).all()
+
+
+def test_alternatives_whose_quotients_are_subnormal(cuda_lib, rng):
+    """At temperatures that leave a quotient few bits, many different logits share one and go by their indices."""
+    for rows, n in ((4, 900), (2, 70001)):
+        x = torch.from_numpy(rng.standard_normal((rows, n)) * 2).float().cuda()
+        for temp in (1e30, 1e37, 3e38):
+            xs = (x * 1e-7 if temp > 1e36 else x).cpu().numpy()
+            z = xs / np.float32(temp)
+            got = run(torch.from_numpy(xs).cuda(), None, 32, temp)
+            assert np.array_equal(got["top_ids"], np.argsort(-z, axis=1, kind="stable")[:, :32]), temp
+
+
 def test_peaked_rows_keep_their_small_numbers(cuda_lib):
     """Where nearly all probability is on one token, its log probability and the entropy are far below 1 and keep
     their leading digits: relative error of the sums 2^-24 (n / 128 + 64), of e^u 2^-23 (|u| + 2)."""
