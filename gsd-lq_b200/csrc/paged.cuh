@@ -4,6 +4,10 @@
 
 namespace gsdlq {
 
+// Positions above it are refused, so that a row's length rounded up to whole tiles stays within an int, whatever the
+// table allows.
+constexpr int PAGED_MAX_POS = INT32_MAX - 128;
+
 // Sequence of row r, and how many positions it has with its own (0: idle).  `flag`: report what is wrong
 // with it (once per launch is enough).
 struct PagedRow {
@@ -17,7 +21,7 @@ __device__ __forceinline__ PagedRow paged_row(const gsdlq_paged_kv_t& kv, const 
     if (flag) raise_flag(GSDLQ_FLAG_BAD_PAGE);
     return {s, 0};
   }
-  if (p < 0 || (long long)p >= (long long)kv.max_blocks * kv.page_size) {
+  if (p < 0 || p > PAGED_MAX_POS || (long long)p >= (long long)kv.max_blocks * kv.page_size) {
     if (flag) raise_flag(GSDLQ_FLAG_BAD_POS);
     return {s, 0};
   }

@@ -448,9 +448,9 @@ int gsdlq_argmax_rows(const float *logits, int rows, int n, int *ids, int *pos, 
  * Rows: the per-row calls take `rows` new tokens.  Row r belongs to sequence row_seq[r] (row_seq
  * NULL: sequence r) and stands at position pos[r]; pos[r] = -1 is an idle row (nothing is stored,
  * its attention output is zero).  One row per sequence is a decode step; consecutive positions of
- * one sequence are a chunk of its prompt.  Positions below -1 or at max_blocks * page_size and
- * above set GSDLQ_FLAG_BAD_POS, sequence indices outside [0, n_seqs) GSDLQ_FLAG_BAD_PAGE; such rows
- * are treated as idle.  Arrays of one call must not overlap unless said so. */
+ * one sequence are a chunk of its prompt.  Positions below -1, at max_blocks * page_size and above, or
+ * above 2^31 - 129 set GSDLQ_FLAG_BAD_POS, sequence indices outside [0, n_seqs) GSDLQ_FLAG_BAD_PAGE;
+ * such rows are treated as idle.  Arrays of one call must not overlap unless said so. */
 #define GSDLQ_KV_F16 0
 #define GSDLQ_KV_BF16 1
 #define GSDLQ_PAGED_MAX_SEQS 1024 /* largest n_seqs, and largest rows of gsdlq_pages_reserve */

@@ -469,6 +469,55 @@ def test_pages_bad_entries_are_reported_and_harmless(cuda_lib):
     assert torch.equal(kv.k, want) and flags() == []
 
 
+def test_positions_next_to_the_end_of_32_bits(cuda_lib, rng):
+    """Tables that reach past 2^31 positions: the last positions are refused by every call, those before them are not,
+    and the other rows of the call are as they are without them."""
+    import ctypes
+
+    import gsdlq_b200._lib as L
+    from gsdlq_b200 import ops, paged
+    page, top = 1 << 30, 2**31 - 129
+    table, refs = dev([[-1] * 3, [-1] * 3]), dev([0] * 4)
+    desc = L.PagedKVDesc(kv_type=0, layers=1, n_pages=4, page_size=page, n_kv_heads=1, head_dim=32,
+                         table=table.data_ptr(), refs=refs.data_ptr(), n_seqs=2, max_blocks=3)  # (no pool is looked at)
+    src, dst, counts = dev([-1] * 4), dev([-1] * 4), dev([0] * 4)
+
+    def reserve(pos):
+        p = dev(pos)
+        assert cuda_lib.gsdlq_pages_reserve(ctypes.byref(desc), None, p.data_ptr(), 2, src.data_ptr(), dst.data_ptr(), 2,
+                                            counts.data_ptr(), ops._stream_on(p.device)) == 0
+        return counts[:3].tolist()
+
+    assert reserve([top, 5]) == [0, 0, 2] and table.tolist() == [[-1, 0, -1], [1, -1, -1]] and flags() == []
+    assert reserve([2**31 - 1, top + 1]) == [0, 0, 0] and flags() == ["bad_pos"]
+    # a table of 2^31 + 64 positions over a small pool
+    small = make_pool(rng, [40], 16, 1, 64, torch.float16)
+    table = torch.full((1, (1 << 27) + 4), -1, dtype=torch.int32, device="cuda")
+    table[0, :3] = small.table[0, :3]
+    kv = paged.PagedKV.wrap(small.k, small.v, table, small.refs)
+    rows = [39, 2**31 - 1, top + 1, 7]
+    for pos in (rows, rows[1:] + rows[:1]):
+        q = torch.from_numpy(rng.standard_normal((len(pos), 2, 64))).float().cuda()
+        got = run_attention(kv, 0, q, pos, [0] * len(pos))
+        assert flags() == ["bad_pos"]
+        for r, p in enumerate(pos):
+            if p > top:
+                assert not got[r].any()
+                continue
+            k, v = rows_of(kv, 0, 0, p + 1)
+            want, tol = O.attention(q[r].cpu().numpy(), k, v, 0.125)
+            assert (np.abs(got[r] - want) <= tol).all()
+    with pytest.raises(L.GsdlqError, match="unsupported"):  # (enough rows to share tiles are too many for such a table)
+        run_attention(kv, 0, torch.zeros(128, 2, 64, device="cuda"), rows * 32, [0] * 128)
+    cs = torch.zeros(64, 32, 2, device="cuda")
+    before = kv.k.clone()
+    x = torch.ones(1, 2, 64, device="cuda")
+    out = torch.zeros_like(x)
+    ops.rope_kv_paged(ops.paged_append_job(kv, 0, x, x[:, :1], x[:, :1], out, dev([2**31 - 1]), cs))
+    assert torch.equal(out, x) and torch.equal(kv.k.view(torch.int16), before.view(torch.int16))
+    assert flags() == ["bad_pos"]
+
+
 def test_resized_pool(cuda_lib):
     kv = empty_pool(12, 4, 3, 3)
     kv.reserve(dev([0, 4, 8]))
