@@ -418,6 +418,7 @@ int gsdlq_rope_kv_paged(const gsdlq_paged_append_job_t* job, gsdlq_stream_t stre
   if (!job || !pool_ok(job->kv) || !rows_ok(job->kv, job->row_seq, job->pos, job->rows)) return GSDLQ_ERR_INVALID;
   const gsdlq_paged_append_job_t& J = *job;
   if (!J.q || !J.k || !J.v || !J.q_out || !J.rope_cs || J.max_pos <= 0 || J.n_heads <= 0) return GSDLQ_ERR_INVALID;
+  if (reinterpret_cast<uintptr_t>(J.rope_cs) & 7u) return GSDLQ_ERR_INVALID;  // read in pairs
   if (J.layer < 0 || J.layer >= J.kv.layers) return GSDLQ_ERR_INVALID;
   const long long qw = (long long)J.n_heads * J.kv.head_dim, kw = (long long)J.kv.n_kv_heads * J.kv.head_dim;
   if (qw > INT32_MAX / 4 || kw > INT32_MAX / 4) return GSDLQ_ERR_INVALID;

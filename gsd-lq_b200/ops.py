@@ -335,6 +335,8 @@ def paged_append_job(kv, layer: int, q, k, v, q_out, pos, rope_cs, row_seq=None,
     if _row_stride(k) != _row_stride(v):
         raise ValueError("k and v must have the same row stride")
     _check(rope_cs, "rope_cs", torch.float32, (None, hd // 2, 2), dev)
+    if rope_cs.data_ptr() % 8:
+        raise ValueError("rope_cs must start at a multiple of 8 bytes")
     if not 0 <= layer < kv.n_layers:
         raise ValueError(f"layer outside [0, {kv.n_layers})")
     j = L.PagedAppendJob(kv=kv.desc(), layer=layer, q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(),

@@ -475,7 +475,7 @@ typedef struct gsdlq_paged_append_job {
   const float *q, *k, *v; /* rows of [n_heads][head_dim] and [n_kv_heads][head_dim]                   */
   float *q_out;           /* rotated q; may be q itself (same stride)                                 */
   int q_stride, kv_stride, q_out_stride; /* elements between rows; 0: packed                          */
-  const float *rope_cs;   /* [max_pos][head_dim/2] (cos, sin) pairs                                   */
+  const float *rope_cs;   /* [max_pos][head_dim/2] (cos, sin) pairs, 8-byte aligned                   */
   int max_pos;            /* positions at and above it: GSDLQ_FLAG_BAD_POS, treated as idle           */
   int interleaved;        /* 1: pairs (2i, 2i+1); 0: (i, i + head_dim/2)                              */
   const int *row_seq, *pos;

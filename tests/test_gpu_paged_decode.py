@@ -324,3 +324,15 @@ def test_wrong_tensors_are_refused(cuda_lib):
     small = ops.paged_attn_job(kv, 0, q, f(3, 4, 64), pos, 0.125, work[:64])
     with pytest.raises(Exception, match="invalid argument"):
         ops.attention_paged(small)
+
+
+def test_angles_off_their_pairs_are_refused(cuda_lib):
+    """By the job, so that no launch is made with them."""
+    from gsdlq_b200 import ops, paged
+    kv = paged.PagedKV(1, 8, 16, 2, 64, 3, 4)
+    q, k = torch.zeros(3, 4, 64, device="cuda"), torch.zeros(3, 2, 64, device="cuda")
+    pos = torch.zeros(3, dtype=torch.int32, device="cuda")
+    flat = torch.zeros(64 * 64 + 2, device="cuda")
+    ops.paged_append_job(kv, 0, q, k, k, q, pos, flat[2:].view(64, 32, 2))
+    with pytest.raises(ValueError, match="rope_cs"):
+        ops.paged_append_job(kv, 0, q, k, k, q, pos, flat[1:-1].view(64, 32, 2))

@@ -196,3 +196,12 @@ def test_attention_work_serves_every_shape_in_turn():
              for rows, heads, kv_heads, hd in ((1, 4, 4, 32), (128, 32, 32, 64), (300, 32, 8, 128), (2, 2, 1, 64))}
     assert len(parts) == 1
     assert all(size(r, 32, 8, 64) <= size(r + 1, 32, 8, 64) for r in range(1, 70))
+
+
+def test_append_refuses_angles_off_their_pairs():
+    """The angles are read in pairs, so a table that starts at an odd element is refused before any launch."""
+    lib = L.load()
+    for off in (4, 12, 1):
+        job = L.PagedAppendJob(kv=kv(), layer=1, q=A, k=A, v=A, q_out=A, rope_cs=A + off, max_pos=80, interleaved=1, pos=A,
+                               rows=4, n_heads=4)
+        assert lib.gsdlq_rope_kv_paged(ctypes.byref(job), None) == -1
