@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cfloat>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -255,12 +256,67 @@ struct PaColumns {
       acc[n + 1][1] = fmaf(acc[n + 1][1], W.f, o1[1] + o1[3]);
     }
   }
+  // What values() of a tile without its non-finite entries (pa_finite) leaves out: those of the positions `mine`, into
+  // their own dimensions.
+  template <typename M>
+  __device__ __forceinline__ void add_not_finite(const uint8_t* tile, M mine) {
+    for (int j = 0; j < TOK; ++j) {
+      if (!((mine >> j) & 1)) continue;
+#pragma unroll
+      for (int n = 0; n < CH; ++n) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + pa_at<HD>(j, n) + 4 * (threadIdx.x & 3));
+        float2 f;
+        if constexpr (BF16) {
+          f = make_float2(bf16lo_to_f(w), bf16hi_to_f(w));
+        } else {
+          f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        }
+        if (!isfinite(f.x)) acc[n][0] += f.x;
+        if (!isfinite(f.y)) acc[n][1] += f.y;
+      }
+    }
+  }
   // this lane's sums over its column's four lanes
   __device__ __forceinline__ void finish() {
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
   }
 };
+// Those of the positions lo .. hi - 1 of a tile (and their neighbours) that hold entries that are not finite (exponent all
+// ones); if there are any, `to` receives the tile with zeros for them.
+template <int HD, bool BF16, typename M>
+__device__ __forceinline__ M pa_finite(const uint8_t* tile, int lo, int hi, uint8_t* to) {
+  constexpr int CH = HD / 8, POS = 32 / CH, STEPS = pa_tok(HD) / POS;  // CH lanes a position
+  constexpr uint32_t E = BF16 ? 0x7f807f80u : 0x7c007c00u, ONE = BF16 ? 0x00800080u : 0x04000400u;
+  const int lane = threadIdx.x & 31, s0 = lo / POS, s1 = (hi + POS - 1) / POS;
+  const uint4* const at = reinterpret_cast<const uint4*>(tile) + lane;
+  auto test = [](uint32_t w) { return ((w & E) + ONE) & 0x80008000u; };  // the upper bit of each such half
+  uint32_t any = 0u;
+#pragma unroll 2
+  for (int it = s0; it < s1; ++it) {
+    const uint4 w = at[it * 32];
+    any |= test(w.x) | test(w.y) | test(w.z) | test(w.w);
+  }
+  if (!__any_sync(0xffffffffu, any)) return 0;
+  M bad = 0;
+  __syncwarp();  // what the lanes read of `to` before
+#pragma unroll 1
+  for (int it = 0; it < STEPS; ++it) {
+    uint4 w = at[it * 32];
+    if (it >= s0 && it < s1) {
+      const uint32_t x = test(w.x), y = test(w.y), z = test(w.z), u = test(w.w);
+      const unsigned b = __ballot_sync(0xffffffffu, x | y | z | u);
+      for (int i = 0; i < POS; ++i)
+        if ((b >> (i * CH)) & ((1u << CH) - 1u)) bad |= (M)1 << (it * POS + i);
+      w = make_uint4(w.x & ~((x >> 15) * 0xffffu), w.y & ~((y >> 15) * 0xffffu), w.z & ~((z >> 15) * 0xffffu),
+                     w.w & ~((u >> 15) * 0xffffu));
+    }
+    reinterpret_cast<uint4*>(to)[it * 32 + lane] = w;
+  }
+  __syncwarp();
+  return bad;
+}
+
 __device__ __forceinline__ float pa_inverse(float x) { return x > 0.f ? 1.f / x : (x == 0.f ? 0.f : NAN); }  // 0: no position left
 
 // One thread, after a barrier behind which the CTA's part is written: whether it is the last of n_parts CTAs, whose
@@ -719,12 +775,17 @@ constexpr int PC_OVER = 2;    // units that an item counts besides its own (thos
 template <int HD>
 struct PagedChunkSmem {
   uint8_t tile[PC_STAGES][2][pa_tok(HD) * HD * 2];  // K, V
-  unsigned valid[PC_STAGES][PA_WARPS];              // of the positions that a warp has looked up
-  float f[PA_WARPS][PA_GROUP][PA_MAX_CTAS];         // the parts' factors, while they are joined
+  // the parts' factors, while they are joined; before that each warp's copy of a tile of V without what is not finite
+  alignas(1024) float f[PA_WARPS][PA_GROUP][PA_MAX_CTAS];
+  unsigned long long bad[PA_WARPS];     // positions whose entries of V are not all finite, of a warp's tile
+  unsigned valid[PC_STAGES][PA_WARPS];  // of the positions that a warp has looked up
   int seq[PA_THREADS], len[PA_THREADS];             // of the rows, while the packs are counted
   int warp_sum[PA_WARPS];
   int row, base, last;
 };
+
+static_assert(sizeof(float) * PA_GROUP * PA_MAX_CTAS % 1024 == 0 && sizeof(float) * PA_GROUP * PA_MAX_CTAS >= 32 * 128 * 2,
+              "a warp's copy of a tile: its size and alignment");
 
 struct PagedPack {
   int row, n, seq, len, tiles;  // its rows, their sequence, the longest one's positions and units
@@ -922,8 +983,11 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
     gq = min(PA_GROUP, gq_all - sub * PA_GROUP);
     return g * gq_all + sub * PA_GROUP;
   };
+  int least = 0, most = 0;  // positions of the warp's shortest row (idle ones apart) and of its longest
   auto next_seg = [&]() {
     if (!advance(cur)) return false;
+    least = __reduce_min_sync(0xffffffffu, cur.own > 0 ? cur.own : INT_MAX);
+    most = __reduce_max_sync(0xffffffffu, cur.own);
     int gq;
     const int head0 = first_head(cur, gq);
     // (columns without a row or a head of their own repeat another's)
@@ -953,7 +1017,17 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
       copy(U, stage == 0 ? PC_STAGES - 1 : stage - 1);
       look(U);
       const int limit = cur.own - cur.t * TOK;  // positions of the tile that this lane's row has
-      if (__any_sync(0xffffffffu, limit > 0)) {
+      if (cur.t * TOK < most) {
+        // Positions of the tile behind a row's end that other rows of the pack use must not reach its sums, not even as 0
+        // times what is not finite: the product is taken without such entries, and the rows that use them add them.
+        uint8_t* const clean = reinterpret_cast<uint8_t*>(S.f[warp]);
+        bool wild = false;
+        if (least < min(cur.t * TOK + TOK, cur.len)) {
+          const mask_t bad = pa_finite<HD, BF16, mask_t>(S.tile[stage][1], max(least - cur.t * TOK, 0),
+                                                         min(cur.len - cur.t * TOK, TOK), clean);
+          wild = bad != 0;
+          if (wild) S.bad[warp] = bad;  // (not kept in registers through the products: they would spill)
+        }
         const uint32_t k0 = tiles + stage * 2 * TILE + pa_at<HD>(lane & 7, lane >> 3);
         const uint32_t v0s = tiles + stage * 2 * TILE + TILE + pa_at<HD>(lane & 15, lane >> 4);
         float p[TOK / 8][2];
@@ -972,12 +1046,17 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
         }
         typename Cols::Weights W;
         C.weights(W, p);
-        C.values(W, v0s);
+        C.values(W, !wild ? v0s : smem_u32(clean) + pa_at<HD>(lane & 15, lane >> 4));
+        if (wild) C.add_not_finite(S.tile[stage][1], (mask_t)S.bad[warp] & valid);
       }
       stage = stage + 1 == PC_STAGES ? 0 : stage + 1;
     }
     // ---- the segment's result, each warp its rows'
     C.finish();
+    if (C.l == 0.f) {  // no position: zeros, also for an idle row among others whose values are not finite
+#pragma unroll
+      for (int n = 0; n < CH; ++n) C.acc[n][0] = C.acc[n][1] = 0.f;
+    }
     int gq;
     const int head0 = first_head(cur, gq), h = lane >> 2;
     const bool mine = rl < rows_warp && hl < gq && warp * rows_warp + rl < cur.n;

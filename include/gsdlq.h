@@ -487,8 +487,9 @@ int gsdlq_rope_kv_paged(const gsdlq_paged_append_job_t *job, gsdlq_stream_t stre
  * out[r][h] = sum_t p_t V[t], p = softmax_t(sm_scale * q[r][h] . K[t]), with kv head
  * h / (n_heads / n_kv_heads) -- gsd_cpu_gqa_attention (gsd_lq_cpu_engine.c:265-330) per row.  Any
  * n_heads that is a multiple of n_kv_heads.  Positions whose page is missing are left out
- * (GSDLQ_FLAG_BAD_PAGE); a row with no position left gives zeros.  Cache rows in use and q must be
- * finite; what lies behind pos[r] in a page is never used, whatever it holds.
+ * (GSDLQ_FLAG_BAD_PAGE); a row with no position left gives zeros.  q and the cache rows of positions
+ * 0 .. pos[r] must be finite for row r's result to be; what lies behind pos[r] never reaches it,
+ * whatever it holds and whichever other rows of the call use it.
  * work: gsdlq_attention_paged_work_size bytes, 16-byte aligned, all zero before its first use; each
  * launch leaves it as the next one needs it, so one area serves launches of different rows, heads and
  * head sizes in turn, if it has the largest of their sizes (a size grows with rows * n_kv_heads).

@@ -148,6 +148,59 @@ def test_attention_chunks_over_long_caches(cuda_lib, rng):
             check_attention(kv, 0, q, pos, [0] * rows)
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("hd,nkv,group,page", [(128, 2, 6, 16), (64, 32, 1, 16), (32, 8, 2, 5), (128, 8, 4, 48)])
+def test_a_row_never_meets_what_lies_behind_it(cuda_lib, rng, kind, hd, nkv, group, page):
+    """Cache rows that are not finite, in use by later rows of the call: the rows before them, in the same pack of rows
+    and elsewhere, are as they are without; idle rows among them are zero."""
+    n = 2100
+    kv = make_pool(rng, [n], page, nkv, hd, DTYPES[kind])
+    k, v = rows_of(kv, 0, 0, n)
+    wild = {1300: math.inf, 2040: -math.inf, 2041: math.nan, 2063: math.inf, 2095: math.nan}
+    for t, x in wild.items():
+        at = (0, int(kv.table[0, t // page]), t % page, int(rng.integers(0, nkv)), int(rng.integers(0, hd)))
+        kv.v[at] = x
+        if t % 2:
+            kv.k[at] = x
+    from gsdlq_b200 import ops
+
+    def run(q, pos):  # (run_attention's comparison of two launches has no use for NaN)
+        out = torch.full_like(q, 77.0)
+        ops.attention_paged(ops.paged_attn_job(kv, 0, q, out, dev(pos), hd ** -0.5,
+                                               ops.attention_paged_work(kv, len(pos), q.shape[1]), dev([0] * len(pos))))
+        return out.cpu().numpy()
+
+    cases = [list(range(n - 128, n)),                                     # the last chunk of a prompt
+             list(range(1290, 1311)) * 7,                                 # short packs, over again
+             [2039 - r if r % 3 else 2099 - r for r in range(130)],       # ends far apart and in any order
+             [int(p) for p in rng.integers(-1, n, 200)]]                  # idle rows too
+    for pos in cases:
+        q = torch.from_numpy(rng.standard_normal((len(pos), nkv * group, hd)) * 2).float().cuda()
+        for rows in (slice(None), slice(0, 2)):  # tiles shared by many rows, and a tile per row
+            got = run(q[rows], pos[rows])
+            clean = [r for r, p in enumerate(pos[rows]) if p < 1300]
+            assert np.isfinite(got[clean]).all()
+            for r in clean[::8]:
+                p = pos[r]
+                want, tol = O.attention(q[r].cpu().numpy(), k[:p + 1], v[:p + 1], hd ** -0.5)
+                assert (np.abs(got[r] - want) <= tol).all(), (r, p)
+    # the first of them gone: the rows up to the second
+    at = (0, int(kv.table[0, 1300 // page]), 1300 % page)
+    kv.v[at] = torch.from_numpy(v[1300]).to(kv.v.dtype).cuda()
+    for pos in cases[0], cases[2], cases[3]:
+        q = torch.from_numpy(rng.standard_normal((len(pos), nkv * group, hd)) * 2).float().cuda()
+        got = run(q, pos)
+        for r, p in enumerate(pos):
+            if p < 2040:
+                assert np.isfinite(got[r]).all(), (r, p)
+                if r % 8 == 0 or p > 2030:
+                    want, tol = O.attention(q[r].cpu().numpy(), k[:p + 1], v[:p + 1], hd ** -0.5)
+                    assert (np.abs(got[r] - want) <= tol).all(), (r, p)
+            elif p >= 2041:  # position 2041's NaN in K and V is its own
+                assert np.isnan(got[r]).any(), (r, p)
+    assert flags() == []
+
+
 def test_one_work_area_serves_launches_of_any_shape_in_turn(cuda_lib, rng):
     """Launches of few and many rows, in both forms and of all head sizes, on one work area: each the same bit for bit
     as with a work area of its own, with every row written, and within the bound."""
