@@ -207,7 +207,14 @@ class BatchDecoder:
     def logprobs(self, ids=None, top: int = 0, temperature: float = 1.0) -> dict:
         """Of the last step's logits, per sequence (gsdlq_logprobs_rows): the entropy, the log probability of
         the given token ids (default: the greedy picks), and the ``top`` most likely tokens with theirs."""
-        return self.m._logprobs(self.logits, self.ids if ids is None else ids, top, temperature)
+        return self.m._logprobs(self.logits, self._picks() if ids is None else ids, top, temperature)
+
+    def _picks(self) -> torch.Tensor:
+        """The greedy picks of the last step's logits (self.ids are the next inputs, which may be others by now)."""
+        picks = torch.empty_like(self.ids)
+        L.check(L.load().gsdlq_argmax_rows(self.logits.data_ptr(), self.B, self.m.vocab_local, picks.data_ptr(), None,
+                                           None, 0, ops.stream_handle()), "gsdlq_argmax_rows")
+        return picks
 
     def generate(self, prompts, max_new_tokens: int) -> list[list[int]]:
         """Greedy continuation of every prompt (prefilled by chunks, then lockstep decode)."""

@@ -336,3 +336,34 @@ def test_angles_off_their_pairs_are_refused(cuda_lib):
     ops.paged_append_job(kv, 0, q, k, k, q, pos, flat[2:].view(64, 32, 2))
     with pytest.raises(ValueError, match="rope_cs"):
         ops.paged_append_job(kv, 0, q, k, k, q, pos, flat[1:-1].view(64, 32, 2))
+
+
+def test_logprobs_are_the_picks_whatever_the_next_inputs_are(cuda_lib):
+    """Without token ids: those of the logits' best tokens, after a step, after the next tokens were set, after the
+    logits of set tokens without a pick, and after a fork."""
+    import gsdlq_b200._lib as L
+    from gsdlq_b200.batch import BatchDecoder
+    from gsdlq_b200.paged import PagedBatchDecoder
+    m, cfg = model("smollm2-1.7b", "turbo", n_layers=1)
+
+    def check(d):
+        want = log_softmax(d.logits_host())
+        assert np.abs(d.logprobs()["logprob"] - want.max(1)).max() < 1e-4
+        own = d.logprobs([7] * d.B)["logprob"]
+        assert np.abs(own - want[:, 7]).max() < 1e-4
+
+    for d in (BatchDecoder(m, 3, max_seq=64), PagedBatchDecoder(m, 3, 12, 16, max_seq=64)):
+        d.set_tokens([5, 6, 7], [0, 0, 0])
+        d.step()
+        check(d)
+        d.set_tokens([11, 12, 13], [1, 1, 1])
+        check(d)
+        if isinstance(d, PagedBatchDecoder):
+            d.step_logits()
+            assert d.ids.tolist() == [11, 12, 13] and d.pos.tolist() == [1, 1, 1]
+            check(d)
+            d.fork([2, 2, 0])
+            check(d)
+        d.release()
+    assert L.device_flags() == 0
+    m.release()
