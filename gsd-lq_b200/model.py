@@ -752,7 +752,7 @@ class GSDLQModel:
         if self.tp is not None:
             torch.cuda.synchronize(self.device)
             self.tp.close()
-        for k in ("hex", "embed", "norms", "k_cache", "v_cache", "_arena"):
+        for k in ("hex", "embed", "norms", "k_cache", "v_cache", "_arena", "_score_logits"):
             if hasattr(self, k):
                 delattr(self, k)
         torch.cuda.empty_cache()

@@ -202,3 +202,12 @@ def test_generate_refuses_bad_arguments_before_the_device():
             gen(m, [1, 2], 4, start_pos=sp)
     with pytest.raises(NotImplementedError, match="whole vocabulary"):
         gen(types.SimpleNamespace(max_seq=32, tp=object()), [1, 2], 4, temperature=0.7)
+
+
+def test_release_drops_the_logits_that_scoring_keeps():
+    from gsdlq_b200.model import GSDLQModel
+    m = GSDLQModel.__new__(GSDLQModel)
+    m._graphs, m.tp, m._destroy_plans = {}, None, lambda: None
+    m._score_logits = torch.zeros(4)
+    m.release()
+    assert not hasattr(m, "_score_logits")
