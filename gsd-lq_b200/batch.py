@@ -216,15 +216,21 @@ class BatchDecoder:
                                            None, 0, ops.stream_handle()), "gsdlq_argmax_rows")
         return picks
 
-    def generate(self, prompts, max_new_tokens: int) -> list[list[int]]:
-        """Greedy continuation of every prompt (prefilled by chunks, then lockstep decode)."""
+    def _check_prompts(self, prompts, max_new_tokens: int):
         if len(prompts) != self.B:
             raise ValueError(f"{self.B} prompts expected")
-        for b, pr in enumerate(prompts):
+        for pr in prompts:
             if len(pr) == 0:
                 raise ValueError("every prompt needs at least one token")
             if len(pr) + max_new_tokens > self.S:
                 raise ValueError("prompt + new tokens exceed max_seq")
+            if not 0 <= int(pr[-1]) < self.m.vocab_size:
+                raise ValueError("token id outside the vocabulary")
+
+    def generate(self, prompts, max_new_tokens: int) -> list[list[int]]:
+        """Greedy continuation of every prompt (prefilled by chunks, then lockstep decode)."""
+        self._check_prompts(prompts, max_new_tokens)
+        for b, pr in enumerate(prompts):
             self.prefill(b, pr[:-1])
         self.set_tokens([pr[-1] for pr in prompts], [len(pr) - 1 for pr in prompts])
         for _ in range(max_new_tokens):

@@ -291,18 +291,17 @@ class PagedBatchDecoder(BatchDecoder):
         self.fork([-1 if b in gone else b for b in range(self.B)])
 
     def _room(self, lengths):
-        """Raise MemoryError unless sequences of the given lengths fit the pool beside what the others hold."""
-        ps = self.kv.page_size
-        need, have = sum(-(-n // ps) for n in lengths), self.kv.n_pages - self.kv.pages_in_use()
-        if need > have:
-            raise MemoryError(f"{need} pages needed, {have} free")
+        """Raise MemoryError unless sequences of the given lengths fit the whole pool."""
+        need = sum(-(-n // self.kv.page_size) for n in lengths)
+        if need > self.kv.n_pages:
+            raise MemoryError(f"{need} pages needed, {self.kv.n_pages} in the pool")
 
     def generate(self, prompts, max_new_tokens: int) -> list[list[int]]:
-        """Greedy continuation of every prompt; what the sequences held before is freed."""
-        if len(prompts) != self.B:
-            raise ValueError(f"{self.B} prompts expected")
-        self.free(range(self.B))
+        """Greedy continuation of every prompt; what the sequences held before is freed (not if the call is refused:
+        ValueError, or MemoryError where the pool is too small)."""
+        self._check_prompts(prompts, max_new_tokens)
         self._room([len(pr) + max_new_tokens for pr in prompts])
+        self.free(range(self.B))
         return super().generate(prompts, max_new_tokens)
 
     def beam_search(self, prompt, beams: int, max_new_tokens: int, eos_id: int | None = None):
@@ -315,10 +314,12 @@ class PagedBatchDecoder(BatchDecoder):
             raise ValueError("a prompt of at least one token, and prompt + new tokens within max_seq")
         if not 1 <= beams <= min(self.B, L.MAX_TOP - 1):
             raise ValueError(f"beams outside [1, {min(self.B, L.MAX_TOP - 1)}]")
-        self.free(range(self.B))
+        if not 0 <= prompt[-1] < self.m.vocab_size:
+            raise ValueError("token id outside the vocabulary")
         full = (len(prompt) - 1) // self.kv.page_size
         own = -(-(len(prompt) + max_new_tokens) // self.kv.page_size) - full
         self._room([full * self.kv.page_size] + [own * self.kv.page_size] * (beams + 1))
+        self.free(range(self.B))
         self.prefill(0, prompt[:-1])
         rest = [-1] * (self.B - beams)
         live, done = [([], 0.0)], []

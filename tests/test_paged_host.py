@@ -205,3 +205,27 @@ def test_append_refuses_angles_off_their_pairs():
         job = L.PagedAppendJob(kv=kv(), layer=1, q=A, k=A, v=A, q_out=A, rope_cs=A + off, max_pos=80, interleaved=1, pos=A,
                                rows=4, n_heads=4)
         assert lib.gsdlq_rope_kv_paged(ctypes.byref(job), None) == -1
+
+
+def test_refused_generations_leave_the_sequences_alone():
+    import types
+
+    from gsdlq_b200.paged import PagedBatchDecoder
+    d = PagedBatchDecoder.__new__(PagedBatchDecoder)
+    d.m, d.B, d.S = types.SimpleNamespace(vocab_size=100), 2, 64
+    d.kv = types.SimpleNamespace(n_pages=6, page_size=16, pages_in_use=lambda: 0)
+
+    def touched(*a, **k):
+        raise AssertionError("the sequences were touched")
+
+    d.free = d.fork = d.prefill = d.set_tokens = touched
+    for prompts, n, error in (([[1]], 2, ValueError), ([[1], []], 2, ValueError), ([[1], [2] * 60], 5, ValueError),
+                              ([[1], [2, 100]], 2, ValueError), ([[1] * 40, [2] * 49], 10, MemoryError)):
+        with pytest.raises(error):
+            d.generate(prompts, n)
+    for prompt, beams, n, error in (([], 2, 4, ValueError), ([1], 3, 4, ValueError), ([1], 2, 64, ValueError),
+                                    ([1], 2, 0, ValueError), ([5, -1], 2, 4, ValueError), ([1], 2, 60, MemoryError)):
+        with pytest.raises(error):
+            d.beam_search(prompt, beams, n)
+    with pytest.raises(AssertionError):
+        d.generate([[1], [2]], 3)
