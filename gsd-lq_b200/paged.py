@@ -300,7 +300,7 @@ class PagedBatchDecoder(BatchDecoder):
         """Greedy continuation of every prompt; what the sequences held before is freed (not if the call is refused:
         ValueError, or MemoryError where the pool is too small)."""
         self._check_prompts(prompts, max_new_tokens)
-        self._room([len(pr) + max_new_tokens for pr in prompts])
+        self._room([len(pr) + max_new_tokens - 1 for pr in prompts])  # (the last token is not stored)
         self.free(range(self.B))
         return super().generate(prompts, max_new_tokens)
 
@@ -317,8 +317,8 @@ class PagedBatchDecoder(BatchDecoder):
         if not 0 <= prompt[-1] < self.m.vocab_size:
             raise ValueError("token id outside the vocabulary")
         full = (len(prompt) - 1) // self.kv.page_size
-        own = -(-(len(prompt) + max_new_tokens) // self.kv.page_size) - full
-        self._room([full * self.kv.page_size] + [own * self.kv.page_size] * (beams + 1))
+        own = -(-(len(prompt) + max_new_tokens - 1) // self.kv.page_size) - full  # blocks that the beams write to
+        self._room([full * self.kv.page_size] + [own * self.kv.page_size] * beams)
         self.free(range(self.B))
         self.prefill(0, prompt[:-1])
         rest = [-1] * (self.B - beams)

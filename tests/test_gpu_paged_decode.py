@@ -367,3 +367,27 @@ def test_logprobs_are_the_picks_whatever_the_next_inputs_are(cuda_lib):
         d.release()
     assert L.device_flags() == 0
     m.release()
+
+
+def test_what_just_fits_the_pool_is_not_refused(cuda_lib):
+    """20 prompt tokens and 13 new ones store 32 positions, two pages; three beams share the prompt's full page."""
+    import gsdlq_b200._lib as L
+    from gsdlq_b200.paged import PagedBatchDecoder
+    m, cfg = model("smollm2-1.7b", "turbo", n_layers=1)
+    rng = np.random.default_rng(23)
+    prompts = rng.integers(0, cfg["vocab_size"], (2, 20)).tolist()
+    pd = PagedBatchDecoder(m, 2, 4, 16, max_seq=64)
+    assert [len(x) for x in pd.generate(prompts, 13)] == [13, 13]
+    assert pd.kv.pages_in_use() == 4
+    with pytest.raises(MemoryError):
+        pd.generate(prompts, 14)
+    pd.release()
+    for page, pages, n in ((16, 4, 13), (4, 4 + 3 * 4, 13), (1, 19 + 3 * 13, 13)):
+        pd = PagedBatchDecoder(m, 3, pages, page, max_seq=64)
+        assert [len(t) for t, _ in pd.beam_search(prompts[0], 3, n)] == [n] * 3
+        assert pd.kv.pages_in_use() <= pages
+        with pytest.raises(MemoryError):
+            pd.beam_search(prompts[0], 3, n + 1)
+        pd.release()
+    assert L.device_flags() == 0
+    m.release()
