@@ -424,7 +424,7 @@ int gsdlq_rope_kv_paged(const gsdlq_paged_append_job_t* job, gsdlq_stream_t stre
   if (qw > INT32_MAX / 4 || kw > INT32_MAX / 4) return GSDLQ_ERR_INVALID;
   if ((J.q_stride && J.q_stride < qw) || (J.q_out_stride && J.q_out_stride < qw) || (J.kv_stride && J.kv_stride < kw))
     return GSDLQ_ERR_INVALID;
-  if (J.q == J.q_out && J.q_stride != J.q_out_stride) return GSDLQ_ERR_INVALID;
+  if (J.q == J.q_out && (J.q_stride ? J.q_stride : qw) != (J.q_out_stride ? J.q_out_stride : qw)) return GSDLQ_ERR_INVALID;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int half_shift = J.kv.head_dim == 128 ? 6 : J.kv.head_dim == 64 ? 5 : 4;
   const long long parts = ((qw + 2 * kw) / 2 + RK_THREADS - 1) / RK_THREADS;

@@ -365,6 +365,24 @@ def test_append_rows(cuda_lib, rng, kind, hd, nkv, heads, page):
     assert flags() == []
 
 
+def test_append_in_place_with_the_packed_stride_given_or_not(cuda_lib, rng):
+    """0 and the packed stride are the same stride, also where q is rotated in place."""
+    from gsdlq_b200 import ops
+    kv = make_pool(rng, [20, 20, 20], 16, 2, 64, torch.float16)
+    q0 = torch.from_numpy(rng.standard_normal((3, 4, 64))).float().cuda()
+    k = torch.from_numpy(rng.standard_normal((3, 2, 64))).float().cuda()
+    cs = torch.from_numpy(rng.standard_normal((32, 32, 2))).float().cuda()
+    got = []
+    for q_stride, out_stride in ((0, 0), (0, 256), (256, 0), (256, 256)):
+        q = q0.clone()
+        job = ops.paged_append_job(kv, 0, q, k, k, q, dev([19, 18, 3]), cs)
+        job.q_stride, job.q_out_stride = q_stride, out_stride
+        ops.rope_kv_paged(job)
+        got.append(q)
+    assert all(torch.equal(got[0], x) for x in got[1:]) and not torch.equal(got[0], q0)
+    assert flags() == []
+
+
 def test_append_refuses_shared_and_missing_pages(cuda_lib, rng):
     kv = make_pool(rng, [20, 20, 20, 20], 16, 2, 64, torch.float16)
     kv.refs[int(kv.table[0, 1])] = 2   # shared
