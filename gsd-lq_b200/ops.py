@@ -294,8 +294,12 @@ def _check(t, name: str, dtype, shape, device, row_stride: bool = False):
     return t
 
 
-def _row_stride(t) -> int:
-    return t.stride(0) if t.shape[0] > 1 else 0
+def _row_stride(t, most: int = 2**31 - 1) -> int:
+    """Elements between t's rows, for a descriptor that holds up to ``most`` (an int's)."""
+    n = t.stride(0) if t.shape[0] > 1 else 0
+    if n > most:
+        raise ValueError(f"rows more than {most} elements apart")
+    return n
 
 
 def _ints(t, name: str, device, n: int | None = None) -> int:
@@ -421,7 +425,7 @@ def logprobs_job(logits, ids=None, logprob=None, entropy=None, top_ids=None, top
     if not (temperature > 0.0 and math.isfinite(temperature)):
         raise ValueError("temperature must be positive and finite")
     opt = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    j = L.LogprobsJob(logits=logits.data_ptr(), row_stride=_row_stride(logits), rows=rows, n=n,
+    j = L.LogprobsJob(logits=logits.data_ptr(), row_stride=_row_stride(logits, 2**63 - 1), rows=rows, n=n,
                       temperature=temperature, ids=opt(ids), logprob=opt(logprob), entropy=opt(entropy), top=top,
                       top_ids=opt(top_ids), top_logprobs=opt(top_logprobs))
     j.keep, j.device = (logits, ids, logprob, entropy, top_ids, top_logprobs), dev

@@ -229,3 +229,14 @@ def test_refused_generations_leave_the_sequences_alone():
             d.beam_search(prompt, beams, n)
     with pytest.raises(AssertionError):
         d.generate([[1], [2]], 3)
+
+
+def test_row_strides_past_an_int_are_refused():
+    """The row descriptors hold strides as ints: a wider one must not be cut off."""
+    from gsdlq_b200 import ops
+    t = lambda stride: torch.empty_strided((2, 4), (stride, 1), device="meta")  # noqa: E731
+    assert ops._row_stride(t(2**31 - 1)) == 2**31 - 1 and ops._row_stride(t(2**40)[:1]) == 0
+    for stride in (2**31, 2**32 + 256):
+        with pytest.raises(ValueError, match="apart"):
+            ops._row_stride(t(stride))
+    assert ops._row_stride(t(2**32), 2**63 - 1) == 2**32  # (that of logits is a size_t)
