@@ -504,7 +504,7 @@ typedef struct gsdlq_paged_attn_job {
   float *out;          /* [rows][n_heads][head_dim], 16-byte aligned */
   const int *row_seq, *pos;
   int rows, n_heads;
-  float sm_scale;
+  float sm_scale;      /* finite */
   void *work;
   size_t work_bytes;
 } gsdlq_paged_attn_job_t;

@@ -240,3 +240,13 @@ def test_row_strides_past_an_int_are_refused():
         with pytest.raises(ValueError, match="apart"):
             ops._row_stride(t(stride))
     assert ops._row_stride(t(2**32), 2**63 - 1) == 2**32  # (that of logits is a size_t)
+
+
+def test_attention_refuses_a_scale_that_is_not_finite():
+    """From C too, and where a Python float is past the descriptor's fp32."""
+    lib = L.load()
+    n = ctypes.c_size_t()
+    assert lib.gsdlq_attention_paged_work_size(4, 8, 2, 64, ctypes.byref(n)) == 0
+    for scale in (math.nan, math.inf, -math.inf, 1e39):
+        job = L.PagedAttnJob(kv=kv(), layer=1, q=A, out=A, pos=A, rows=4, n_heads=8, sm_scale=scale, work=A, work_bytes=n.value)
+        assert lib.gsdlq_attention_paged(ctypes.byref(job), None) == -1
