@@ -616,6 +616,8 @@ class GSDLQModel:
             raise ValueError("one token id per row")
         if not 0 <= top <= min(logits.shape[1], L.MAX_TOP):
             raise ValueError(f"top outside [0, {min(logits.shape[1], L.MAX_TOP)}]")
+        if ids.dtype != torch.int32:  # ids past an int's range stay out of the vocabulary
+            ids = ids.clamp(-2, logits.shape[1])
         ids = ids.to(dev, torch.int32)
         f32 = dict(dtype=torch.float32, device=dev)
         out = {"logprob": torch.empty(rows, **f32), "entropy": torch.empty(rows, **f32),

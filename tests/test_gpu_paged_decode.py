@@ -391,3 +391,16 @@ def test_what_just_fits_the_pool_is_not_refused(cuda_lib):
         pd.release()
     assert L.device_flags() == 0
     m.release()
+
+
+def test_token_ids_of_wider_types_are_not_cut_off(cuda_lib):
+    import gsdlq_b200._lib as L
+    from gsdlq_b200.model import GSDLQModel
+    logits = torch.arange(40.0, device="cuda").reshape(4, 10)
+    m = GSDLQModel.__new__(GSDLQModel)
+    got = m._logprobs(logits, torch.tensor([2**32 + 5, -1, 9, -2**40 - 1]), 0, 1.0)["logprob"]
+    assert got[[0, 1, 3]].tolist() == [0, 0, 0] and abs(got[2] - log_softmax(np.arange(10))[9]) < 1e-5
+    assert L.flag_names(L.device_flags()) == ["bad_token"]
+    got = m._logprobs(logits, torch.tensor([5, -1, 9, 0]), 0, 1.0)["logprob"]
+    assert np.abs(got - log_softmax(np.arange(10))[[5, 0, 9, 0]] * [1, 0, 1, 1]).max() < 1e-5
+    assert L.device_flags() == 0
