@@ -1127,8 +1127,9 @@ static int launch_attention_paged(const gsdlq_paged_attn_job_t& J, int subs, cud
   }
   const int grid = std::min(PA_PER_SM * num_sms(), PA_MAX_CTAS);
   const int ps = J.kv.page_size, shift = ps & (ps - 1) ? -1 : __builtin_ctz((unsigned)ps);
-  // Several rows a sequence on average, and enough of them: the tiles are worth sharing.  A CTA's warps without rows
-  // are idle then, and its start and end take 4-5 us more.  One tile per row against shared tiles, us:
+  // Several rows a sequence of the table on average (which rows share one is known on the device only), and enough of
+  // them: the tiles are worth sharing.  A CTA's warps without rows are idle then, and its start and end take 4-5 us
+  // more.  One tile per row against shared tiles, us:
   //   16 sequences of 1500, 32/32 heads of 64: 2 rows each 62 / 73, 3 rows 83 / 76; 32/8 of 128: 3 rows 51 / 49, 8 rows
   //   99 / 45; 12/2 of 128: 3 rows 18.7 / 22.9, 4 rows 23.4 / 22.3; 16/2 of 64: 3 rows 13.5 / 15.9, 4 rows 15.6 / 15.3
   //   one sequence of 1500, 32/32 of 64: 4 rows 14.9 / 13.4; 32/8 of 128: 8 rows 15.3 / 18.9, 16 rows 20.9 / 20.2;

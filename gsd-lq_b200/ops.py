@@ -369,7 +369,11 @@ def attention_paged_work(kv, rows: int, n_heads: int) -> torch.Tensor:
 
 
 def paged_attn_job(kv, layer: int, q, out, pos, sm_scale: float, work, row_seq=None):
-    """Job of attention_paged: q [rows][heads][head_dim] fp32 (rows may be strided), out the same shape, packed."""
+    """Job of attention_paged: q [rows][heads][head_dim] fp32 (rows may be strided), out the same shape, packed.
+
+    Whether neighbouring rows of a sequence share their reads of K and V goes by the rows per sequence of the table.
+    For a chunk of one sequence b out of many, make the job over a cache of that sequence alone, with a row_seq of
+    zeros: PagedKV.wrap(kv.k, kv.v, kv.table[b:b + 1], kv.refs)."""
     dev, hd = kv.k.device, kv.head_dim
     rows = _rows(kv, pos, row_seq, dev)
     _check(q, "q", torch.float32, (rows, None, hd), dev, row_stride=True)

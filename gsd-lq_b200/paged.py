@@ -131,8 +131,8 @@ class PagedKV:
 
     def resized(self, n_pages: int) -> "PagedKV":
         """This cache in a pool of ``n_pages`` pages, larger or (after compact) smaller: a new pool with the pages'
-        contents and counts, and the same table tensor, so that this one must not be used any more.  Waits for the
-        device."""
+        contents and counts, and the same table tensor, so that this one, and the jobs, graphs and decoders made over
+        it, must not be used any more.  Waits for the device."""
         keep = min(int(n_pages), self.n_pages)
         if n_pages < 1:
             raise ValueError("at least one page")

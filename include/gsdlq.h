@@ -493,9 +493,14 @@ int gsdlq_rope_kv_paged(const gsdlq_paged_append_job_t *job, gsdlq_stream_t stre
  * work: gsdlq_attention_paged_work_size bytes, 16-byte aligned, all zero before its first use; each
  * launch leaves it as the next one needs it, so one area serves launches of different rows, heads and
  * head sizes in turn, if it has the largest of their sizes (a size grows with rows * n_kv_heads).
- * Launches that may overlap in time (other streams, graphs that run side by side) need a work area
- * each.  GSDLQ_ERR_UNSUPPORTED: n_pages * page_size above 2^31 - 1, or
- * rows * n_kv_heads * max_blocks * page_size above about 2^35. */
+ * Launches that may overlap in time (other streams, graphs that run side by side) need a work area each.
+ * Rows of one sequence that follow one another share the reads of K and V where row_seq is given, rows is
+ * at least 3 n_seqs (4 n_seqs with more than four query heads per kv head) and rows * n_kv_heads at least
+ * 128; otherwise each row reads them for itself.  The rule sees n_seqs, not the rows' sequences, which are
+ * on the device: pass a chunk of one sequence out of many with a table of its own (kv.table = the
+ * sequence's row, kv.n_seqs = 1, row_seq all 0).  The two forms may differ in a result's last bits.
+ * GSDLQ_ERR_UNSUPPORTED: n_pages * page_size above 2^31 - 1, or rows * n_kv_heads * max_blocks *
+ * page_size above about 2^35. */
 typedef struct gsdlq_paged_attn_job {
   gsdlq_paged_kv_t kv;
   int layer;

@@ -231,6 +231,19 @@ def test_one_work_area_serves_launches_of_any_shape_in_turn(cuda_lib, rng):
     assert flags() == []
 
 
+def test_a_chunk_of_one_sequence_through_a_table_of_its_own(cuda_lib, rng):
+    """As the documents say for one sequence out of many: append and attention over a cache of that sequence alone, which
+    shares pool, table and counts with the others'."""
+    from gsdlq_b200 import paged
+    kv = make_pool(rng, [90, 200, 17, 40], 16, 4, 64, torch.float16)
+    alone = paged.PagedKV.wrap(kv.k, kv.v, kv.table[1:2], kv.refs)
+    pos = list(range(100, 200))
+    append_check(alone, 0, rng, pos, 8, row_seq=[0] * 100)
+    q = torch.from_numpy(rng.standard_normal((100, 8, 64))).float().cuda()
+    check_attention(alone, 0, q, pos, [0] * 100)
+    check_attention(kv, 0, q[-1:].repeat(4, 1, 1), [89, 199, 16, 39])
+
+
 def test_attention_strided_q_and_extreme_scores(cuda_lib, rng):
     kv = make_pool(rng, [50, 200, 7], 16, 2, 64, torch.float16)
     wide = torch.from_numpy(rng.standard_normal((3, 4 * 64 + 20))).float().cuda()
