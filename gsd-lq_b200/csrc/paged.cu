@@ -14,10 +14,11 @@ __device__ __forceinline__ uint16_t kv_round(float v) {
 }
 
 // ---------------------------------------------------------------------------------------
-// RoPE + append.  A thread per pair of one of the row's heads: query heads, then key heads, then value heads.  The
-// chain of look-ups (position, then angle and page, then the page's count) bounds it, so no thread does more than
-// one pair, and q does not wait for the page: 1.6 us for one row of 32 + 8 + 8 heads of 128, 3.8 us for 128 rows of
-// 32 + 32 + 32 heads of 64 (4.4 and 4.6 with a CTA per row).
+// RoPE + append.  A thread per pair of one of the row's heads: query heads, then key heads, then value heads.  Few rows
+// are bound by the chain of look-ups (position, then angle and page, then the page's count), so no thread does more than
+// one pair, and q does not wait for the page: 1.6 us for one row of 32 + 8 + 8 heads of 128 (4.4 with a CTA per row).
+// Many rows are bound by the number of threads, each with look-ups of its own: 1.6 us and 1.5 us for each thousand CTAs,
+// 3.8 us for 128 rows of 32 + 32 + 32 heads of 64 (1536 CTAs; 4.6 with a CTA per row).
 constexpr int RK_THREADS = 256;
 template <bool BF16>
 __global__ void __launch_bounds__(RK_THREADS)

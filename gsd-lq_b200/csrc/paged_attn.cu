@@ -37,8 +37,9 @@ namespace gsdlq {
 //
 // Bound by HBM.  Measured on one B200 (device time, L2 cold): 16 rows x 32 kv heads of 64 over 1025-2047 positions,
 // fp16: 41 us for 195 MB (4.8 TB/s; 5.9 TB/s from the first tile to the last, then 3-4 us of joining); 64 rows x 8 kv
-// heads of 128 over 1-8191 positions, bf16: 54 us for 250 MB; one row x 8 kv heads of 128 over 1537 positions: 9.5 us,
+// heads of 128 over 1-8191 positions, bf16: 53 us for 250 MB; one row x 8 kv heads of 128 over 1537 positions: 9.7 us,
 // of which 2.6 pass before the first tile (positions, table, tile: three dependent look-ups) and 3.5 in the join.
+// Heads of 128 take all 255 registers; in bf16 14 words spill (52 bytes stored, 56 loaded), in fp16 one.
 constexpr int PA_MAX_CTAS = 320;  // largest grid of an attention launch
 constexpr int PA_PER_SM = 2;
 constexpr int PA_GROUP = 8;       // query heads of one kv head taken together
@@ -766,9 +767,10 @@ __global__ void __launch_bounds__(PA_THREADS, PA_PER_SM)
 // row.  A pack is a run of rows with the same sequence inside PA_WARPS * rows_warp rows from a multiple of that
 // on, so that every CTA finds the same packs from a row's neighbours alone.  The units are the tiles up to the
 // longest row's end, dealt to the CTAs as above; a warp passes over those that lie behind all its rows.
-// 128 rows at positions 1024-1151 of one sequence, 12 query and 2 kv heads of 128: 23 us (28 without sharing), of which
+// 128 rows at positions 1024-1151 of one sequence, 12 query and 2 kv heads of 128: 23.6 us (28 without sharing), of which
 // 5 pass before the first tile, 9.5 in eight units a CTA and 5 in writing and joining the parts; the units are bound by
-// the latency of a warp's dependent instructions (issue slots 28 % used, tensor pipe 22 % of active cycles).
+// the latency of a warp's dependent instructions (issue slots 28 % used, tensor pipe 22 % of active cycles).  Looking
+// for entries of V that are not finite, in tiles where a row ends, is 0.2 us of it (up to 5 % with 32/8 heads, in bf16).
 constexpr int PC_STAGES = 4;  // tiles of K and V on their way or in use
 constexpr int PC_OVER = 2;    // units that an item counts besides its own (those 128 rows: 0 26.8 us, 1 25.7, 2 24.9, 4 26.2)
 
