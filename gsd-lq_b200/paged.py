@@ -291,10 +291,14 @@ class PagedBatchDecoder(BatchDecoder):
         self.fork([-1 if b in gone else b for b in range(self.B)])
 
     def _room(self, lengths):
-        """Raise MemoryError unless sequences of the given lengths fit the whole pool."""
-        need = sum(-(-n // self.kv.page_size) for n in lengths)
-        if need > self.kv.n_pages:
-            raise MemoryError(f"{need} pages needed, {self.kv.n_pages} in the pool")
+        """Raise MemoryError unless sequences of the given lengths fit the pool once this decoder's are freed, beside
+        the pages that other tables over it hold (waits for the device)."""
+        kv = self.kv
+        own = kv.table[(kv.table >= 0) & (kv.table < kv.n_pages)].long()
+        mine = torch.zeros_like(kv.refs).scatter_add_(0, own, torch.ones_like(own, dtype=kv.refs.dtype))
+        need, have = sum(-(-n // kv.page_size) for n in lengths), kv.n_pages - int((kv.refs > mine).sum())
+        if need > have:
+            raise MemoryError(f"{need} pages needed, {have} free")
 
     def generate(self, prompts, max_new_tokens: int) -> list[list[int]]:
         """Greedy continuation of every prompt; what the sequences held before is freed (not if the call is refused:

@@ -213,7 +213,8 @@ def test_refused_generations_leave_the_sequences_alone():
     from gsdlq_b200.paged import PagedBatchDecoder
     d = PagedBatchDecoder.__new__(PagedBatchDecoder)
     d.m, d.B, d.S = types.SimpleNamespace(vocab_size=100), 2, 64
-    d.kv = types.SimpleNamespace(n_pages=6, page_size=16, pages_in_use=lambda: 0)
+    table, refs = torch.full((2, 4), -1, dtype=torch.int32), torch.zeros(6, dtype=torch.int32)
+    d.kv = types.SimpleNamespace(n_pages=6, page_size=16, table=table, refs=refs)
 
     def touched(*a, **k):
         raise AssertionError("the sequences were touched")
@@ -250,3 +251,23 @@ def test_attention_refuses_a_scale_that_is_not_finite():
     for scale in (math.nan, math.inf, -math.inf, 1e39):
         job = L.PagedAttnJob(kv=kv(), layer=1, q=A, out=A, pos=A, rows=4, n_heads=8, sm_scale=scale, work=A, work_bytes=n.value)
         assert lib.gsdlq_attention_paged(ctypes.byref(job), None) == -1
+
+
+def test_generations_leave_room_for_other_tables_pages():
+    """Pages that this decoder's own table names are free for a generation; those that others over the pool hold are
+    not, also where this one names them too."""
+    import types
+
+    from gsdlq_b200.paged import PagedBatchDecoder
+    d = PagedBatchDecoder.__new__(PagedBatchDecoder)
+    d.m, d.B, d.S = types.SimpleNamespace(vocab_size=100), 2, 64
+    table = torch.tensor([[0, 1, -1, -1], [0, 3, 99, -1]], dtype=torch.int32)
+
+    def room(refs, pages):
+        d.kv = types.SimpleNamespace(n_pages=6, page_size=16, table=table, refs=torch.tensor(refs, dtype=torch.int32))
+        d._room([pages * 16])
+
+    for refs, have in (([2, 1, 0, 1, 0, 0], 6), ([2, 1, 1, 1, 0, 0], 5), ([3, 1, 1, 2, 0, 4], 2)):
+        room(refs, have)
+        with pytest.raises(MemoryError, match=f"{have} free"):
+            room(refs, have + 1)
