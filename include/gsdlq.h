@@ -527,7 +527,8 @@ int gsdlq_pages_fork(const gsdlq_paged_kv_t *kv, const int *parent, gsdlq_stream
 /* A page to write to for every row's position.  Row by row, in order: a missing page is replaced by a
  * free one; a page that other entries name too is replaced by a free one that is to receive its
  * contents, and the pair goes on the list; a page of one's own is kept.  Free pages are taken in
- * ascending order.  When none is left the row's entry stays as it is (GSDLQ_FLAG_NO_PAGE).
+ * ascending order.  When none is left the row's entry stays as it is (GSDLQ_FLAG_NO_PAGE).  Of several rows
+ * at one table entry the first one acts, and counts.
  * counts[0] = pairs, counts[1] = rows that got no page, counts[2] = pages taken; list entries from
  * counts[0] up to max_pairs are -1.  max_pairs >= rows, rows <= GSDLQ_PAGED_MAX_SEQS. */
 int gsdlq_pages_reserve(const gsdlq_paged_kv_t *kv, const int *row_seq, const int *pos, int rows, int *src, int *dst,
